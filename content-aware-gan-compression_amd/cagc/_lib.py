@@ -99,6 +99,17 @@ _PROTOS = {
     "cagc_parsing_input": [_p, _p, _i, _i, _i, _f, _p, _p, _p],
     "cagc_content_mask_workspace": [_i, _i],
     "cagc_content_mask": [_p, _p, _p, _i, _i, _i, _i, _f, _i, _p],
+    "cagc_rms_norm_fwd": [_p] * 6 + [_i64] * 4 + [_i, _i, _f, _p],
+    "cagc_rms_norm_e4m3": [_p] * 6 + [_i64] * 4 + [_i, _i, _f, _p],
+    "cagc_quantize_rows_e4m3": [_p] * 3 + [_i64] * 3 + [_i, _p],
+    "cagc_rms_norm_bwd_workspace": [_i64, _i64, _i],
+    "cagc_rms_norm_bwd": [_p] * 8 + [_i64] * 5 + [_i, _i, _p],
+    "cagc_gated_linear_workspace": [_p, _p] + [_i64] * 5 + [_i],
+    "cagc_gated_linear_fwd": [_p] * 8 + [_i64] * 5 + [_i, _i, _i, _f, _p],
+    "cagc_gated_linear_bwd_workspace": [_i64] * 3 + [_i] * 4,
+    "cagc_gated_linear_bwd": [_p] * 8 + [_i64] * 6 + [_i, _i, _f, _p],
+    "cagc_grad_norm_workspace": [_p, _i],
+    "cagc_clip_grad_norm": [_p] * 5 + [_i, _i, ctypes.c_double, _i, _p],
 }
 _RESTYPES = {
     "cagc_last_error": ctypes.c_char_p,
@@ -109,6 +120,10 @@ _RESTYPES = {
     "cagc_gemm1x1_packed_elems": _i64,
     "cagc_content_mask_workspace": _i64,
     "cagc_gan_kd_loss_tail_ws_floats": _i64,
+    "cagc_rms_norm_bwd_workspace": _i64,
+    "cagc_gated_linear_workspace": _i64,
+    "cagc_gated_linear_bwd_workspace": _i64,
+    "cagc_grad_norm_workspace": _i64,
 }
 EXPORTS = tuple(_PROTOS)
 
@@ -160,6 +175,21 @@ def ptr(t):
 
 
 DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.float64: 2}     # CAGC_F32 / CAGC_F16 / CAGC_F64
+
+
+# the row-wise and gated operators: CAGC_F32 / CAGC_F16 / CAGC_BF16 / CAGC_E4M3
+ROW_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 3, torch.float8_e4m3fn: 4}
+
+
+def rows_of(t, width):
+    """`t` [..., width] as rows for the row-wise entry points: (tensor [rows, width] with unit stride along a row, elements from row to
+    row).  A view where the strides allow it, else a copy."""
+    r = t.reshape(-1, width) if t.dim() != 2 else t
+    n, s = r.shape[0], r.stride(0)
+    if (width > 1 and r.stride(1) != 1) or (n > 1 and s < width):
+        r = r.contiguous()
+        s = width
+    return r, (s if n > 1 else width)
 
 
 def ptr_any(t):

@@ -16,6 +16,7 @@ from torch.nn import functional as F
 from . import content_mask
 from . import model as M
 from . import prune
+from .op import clip_grad_norm_
 from .op import modconv as mc
 
 
@@ -55,12 +56,15 @@ class KDStep:
 
     def __init__(self, student, teacher, discriminator, lr=0.002, g_reg_every=4, kd_l1_lambda=3.0, mixing=0.9,
                  latent=512, fused_adam=None, parsing_net=None, kd_mode="Output_Only", percept_loss=None,
-                 kd_lpips_lambda=3.0, lpips_image_size=256):
+                 kd_lpips_lambda=3.0, lpips_image_size=256, max_grad_norm=None):
         """parsing_net: callable image-batch -> 19-class logits [B,19,512,512] (or a tuple starting with them, BiSeNet's
         convention).  When given, the content mask is derived on device from the TEACHER's image every step
         (cagc.content_mask, reference train.py:155-158) and the `mask` argument of the step functions may be None.
         kd_mode: 'Output_Only' | 'Intermediate' (train.py:163-169).  percept_loss: optional callable (LPIPS in the
-        reference, train.py:173-182; its weights are not obtainable offline, so it is a hook, off by default)."""
+        reference, train.py:173-182; its weights are not obtainable offline, so it is a hook, off by default).
+        max_grad_norm: every optimiser step first scales its gradients to at most this norm over all parameters together
+        (cagc.op.clip_grad_norm_; under data parallelism the averaged gradients); `last_grad_norm` is the norm before, on
+        the device.  None (the reference's training): gradients as they are."""
         assert kd_mode in ("Output_Only", "Intermediate")
         self.student, self.teacher, self.disc = student, teacher, discriminator
         # frozen use of D (generator step): bypass a DistributedDataParallel wrapper — its reducer expects a gradient for
@@ -82,6 +86,11 @@ class KDStep:
         self.optim = torch.optim.Adam(params, lr=lr * c, betas=(0.0 ** c, 0.99 ** c), **kw)
         self.n_latent = (student.module if hasattr(student, "module") else student).n_latent
         self.phase_timer = None
+        self.max_grad_norm, self.last_grad_norm = max_grad_norm, None
+
+    def _clip(self, params):
+        if self.max_grad_norm is not None:
+            self.last_grad_norm = clip_grad_norm_(params, self.max_grad_norm)
 
     def _mark(self, phase=None):
         if self.phase_timer is not None:
@@ -187,6 +196,7 @@ class KDStep:
         self._mark("train_G_d_forward")      # as in the reference's profiler: D forward + teacher forward + the KD loss
         self.optim.zero_grad(set_to_none=True)
         total.backward()
+        self._clip(self.student.parameters())
         self.optim.step()
         self._mark("train_G_g_backward")
         if total.is_cuda:
@@ -281,6 +291,7 @@ class TrainIteration(KDStep):
         self._mark("train_D_d_forward")
         self.d_optim.zero_grad(set_to_none=True)
         d_loss.backward()
+        self._clip(self.disc.parameters())
         self.d_optim.step()
         self._mark("train_D_d_backward")
         return {"d": d_loss.detach(), "real_score": real_pred.mean().detach(), "fake_score": fake_pred.mean().detach()}
@@ -295,6 +306,7 @@ class TrainIteration(KDStep):
         r1_loss = d_r1_loss(real_pred, real_img)
         self.d_optim.zero_grad(set_to_none=True)
         (self.r1 / 2 * r1_loss * self.d_reg_every + 0 * real_pred[0]).backward()
+        self._clip(self.disc.parameters())
         self.d_optim.step()
         self._mark("reg_D")
         return r1_loss.detach()
@@ -311,6 +323,7 @@ class TrainIteration(KDStep):
         if self.path_batch_shrink:
             weighted = weighted + 0 * fake_img[0, 0, 0, 0]
         weighted.backward()
+        self._clip(self.student.parameters())
         self.optim.step()
         self._mark("reg_G")
         return path_loss.detach(), path_lengths.detach()
@@ -618,6 +631,7 @@ class GraphedKDStep(KDStep):
         with torch.cuda.stream(side):
             for _ in range(3):
                 self._fwd_bwd()
+                self._clip(self._flat_param)
                 self._flat_optim.step()
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
@@ -648,6 +662,7 @@ class GraphedKDStep(KDStep):
                 # in either mode (capture is a property of the stream).
                 with torch.cuda.graph(g, capture_error_mode="thread_local" if self._in_graph_comm else "global"):
                     self.losses = self._fwd_bwd()
+                    self._clip(self._flat_param)      # (the padding between parameters is zero)
                     self._flat_optim.step()
             except Exception as e:      # noqa: BLE001 — whatever invalidated the capture (RCCL refusing to be captured, ...)
                 self._in_graph_comm = False
@@ -662,6 +677,7 @@ class GraphedKDStep(KDStep):
                     self.losses = self._fwd_bwd()
                 self.graph_opt = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(self.graph_opt):
+                    self._clip(self._flat_param)
                     self._flat_optim.step()
             except Exception as e:      # noqa: BLE001
                 torch.cuda.synchronize()

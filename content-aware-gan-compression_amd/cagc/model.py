@@ -19,7 +19,7 @@ import torch
 from torch import autograd, nn
 from torch.nn import functional as F
 
-from .op import FusedLeakyReLU, fused_leaky_relu, upfirdn2d
+from .op import FusedLeakyReLU, fused_leaky_relu, gated_linear, rms_norm, upfirdn2d
 from .op import modconv as mc
 
 
@@ -28,6 +28,18 @@ class PixelNorm(nn.Module):
 
     def forward(self, input):
         return mc.pixel_norm(input)
+
+
+class RMSNorm(nn.Module):
+    """PixelNorm's norm with a weight per channel, over the last dimension; with `residual` it returns (out, input + residual)."""
+
+    def __init__(self, dim, eps=1e-6, weight=True):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(dim)) if weight else None
+        self.eps = eps
+
+    def forward(self, input, residual=None):
+        return rms_norm(input, self.weight, residual=residual, eps=self.eps)
 
 
 def make_kernel(k):
@@ -180,6 +192,26 @@ def invalidate_caches(module):
         for attr in ("_scaled", "_packed", "_wino", "_packed_wino", "_packed_gemm"):
             if getattr(m, attr, None) is not None:
                 setattr(m, attr, None)
+
+
+class GatedLinear(nn.Module):
+    """act(gate) * up of two EqualLinear projections in one kernel: weight [2 out_dim, in_dim], the gate's rows first, with EqualLinear's
+    run-time scale and learning-rate multiplier.  activation: 'silu' or 'gelu'."""
+
+    def __init__(self, in_dim, out_dim, bias=True, lr_mul=1, activation="silu"):
+        super().__init__()
+        self.weight = nn.Parameter(torch.randn(2 * out_dim, in_dim).div_(lr_mul))
+        self.bias = nn.Parameter(torch.zeros(2 * out_dim)) if bias else None
+        self.activation = activation
+        self.scale = (1 / math.sqrt(in_dim)) * lr_mul
+        self.lr_mul = lr_mul
+
+    def forward(self, input):
+        bias = self.bias if self.bias is None or self.lr_mul == 1 else self.bias * self.lr_mul
+        return gated_linear(input, self.weight, bias, activation=self.activation, scale=self.scale)
+
+    def __repr__(self):
+        return f"{self.__class__.__name__}({self.weight.shape[1]}, {self.weight.shape[0] // 2}, activation={self.activation!r})"
 
 
 class ScaledLeakyReLU(nn.Module):

@@ -1,0 +1,390 @@
+// Root-mean-square norm of rows, with the residual's addition before it and, for 8-bit products, e4m3 output with a scale per row.
+//   h = x + residual (rounded to the type: it is an output),  rstd = (mean(h^2) + eps)^-1/2,  y = h rstd w
+//   e4m3: scale = max |y| / 448, q = y / scale
+//   backward, with t = dy w and n = h rstd:  dx = dresidual = rstd (t - n mean(t n)) + dh,   dw = sum over rows of dy n
+//
+// Bound by HBM: a row is read once and kept in registers between its sums and its output (TPR threads a row, NV chunks of 16 bytes each),
+// so a forward moves x, residual, h and y once.  Sums are fp32.  Rows may start at any address: the 16-byte loads need no alignment, only the
+// chunk that crosses a row's end goes element by element.
+#include "common.h"
+
+namespace cagc {
+namespace {
+
+struct __attribute__((packed, aligned(1))) Any16 { uint32_t v[4]; };
+
+template <class T> struct Row { static constexpr int V = 16 / (int)sizeof(T); };
+
+// V elements from p (any alignment) as floats; those from `left` on are zero and not read
+template <int V, class T> __device__ __forceinline__ void load_v(float (&f)[V], const T* p, int64_t left) {
+  T e[V];
+  if (left >= V) {
+    constexpr int N = V * (int)sizeof(T) / 16;
+    static_assert(N >= 1, "whole 16-byte pieces");
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const Any16 a = reinterpret_cast<const Any16*>(p)[i];
+      __builtin_memcpy(reinterpret_cast<char*>(e) + 16 * i, &a, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = (float)e[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i < left ? (float)p[i] : 0.f;
+  }
+}
+template <int V, class T> __device__ __forceinline__ void store_v(T* p, const float (&f)[V], int64_t left) {
+  if (left >= V) {
+    T e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = (T)f[i];
+    Any16 a;
+    static_assert(V * sizeof(T) == 16, "one 16-byte piece");
+    __builtin_memcpy(&a, e, 16);
+    *reinterpret_cast<Any16*>(p) = a;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (i < left) p[i] = (T)f[i];
+  }
+}
+// V e4m3 bytes
+template <int V> __device__ __forceinline__ void store_q(uint8_t* p, const float (&f)[V], float inv, int64_t left) {
+  uint32_t d[V / 4];
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) {
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inv, f[4 * i + 1] * inv, 0, false);
+    d[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, v, true);
+  }
+  struct __attribute__((packed, aligned(1))) Any { uint32_t v[V / 4]; };
+  if (left >= V) {
+    Any a;
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) a.v[i] = d[i];
+    *reinterpret_cast<Any*>(p) = a;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (i < left) p[i] = (uint8_t)(d[i / 4] >> (8 * (i & 3)));
+  }
+}
+
+// sum / largest over the TPR threads of a row; every thread gets it.  `sh`: TPR / 64 words of this row's own, one use a call.
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float* sh) {
+  v = wave_sum(v);
+  if (TPR == 64) return v;
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < TPR / 64; ++i) s += sh[i];
+  return s;
+}
+// magnitudes compared as bit patterns: a NaN is above infinity and so is kept
+template <int TPR> __device__ __forceinline__ float row_top(uint32_t v, uint32_t* sh) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, 64));
+  if (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) v = max(v, sh[i]);
+  }
+  return __builtin_bit_cast(float, v);
+}
+
+struct Norm {
+  void* y;               // [rows, dim]: the element type, or e4m3
+  float* scale;          // [rows] (e4m3)
+  void* h;               // [rows, dim] [nullable]
+  float* rstd;           // [rows] [nullable]
+  const void* x;
+  const void* res;       // [nullable]
+  const void* w;         // [dim] [nullable]
+  int64_t rows, xs, rs;  // rows of x and residual are xs, rs elements apart
+  int dim;
+  float eps;
+};
+
+// OUT: 0 = the element type, 1 = e4m3, 2 = e4m3 of the rows themselves, without the norm
+template <class T, class W, int TPR, int NV, int OUT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(Norm a) {
+  constexpr int V = Row<T>::V, RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float sh[2][TPR / 64];
+  const int t = threadIdx.x % TPR;
+  const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (r >= a.rows) return;                     // (a whole wave, and with more than 64 threads a row the whole workgroup)
+  const T* x = static_cast<const T*>(a.x) + r * a.xs;
+  const T* res = a.res ? static_cast<const T*>(a.res) + r * a.rs : nullptr;
+  T* h = a.h ? static_cast<T*>(a.h) + r * a.dim : nullptr;
+  float v[NV][V], ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < NV; ++c) load_v<V>(v[c], x + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+  if (res) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      float f[V];
+      load_v<V>(f, res + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[c][i] = (float)(T)(v[c][i] + f[i]);
+    }
+  }
+  if (h) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c) store_v<V>(h + (t + c * TPR) * V, v[c], a.dim - (t + c * TPR) * V);
+  }
+  if (OUT != 2) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) ss += v[c][i] * v[c][i];
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, sh[0]) / (float)a.dim + a.eps);
+    if (a.rstd && t == 0) a.rstd[r] = rstd;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      if (a.w) {
+        float f[V];
+        load_v<V>(f, static_cast<const W*>(a.w) + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[c][i] *= rstd * f[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[c][i] *= rstd;
+      }
+    }
+  }
+  if (OUT == 0) {
+    T* y = static_cast<T*>(a.y) + r * a.dim;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) store_v<V>(y + (t + c * TPR) * V, v[c], a.dim - (t + c * TPR) * V);
+    return;
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[c][i]) & 0x7fffffffu);
+  const float most = row_top<TPR>(top, reinterpret_cast<uint32_t*>(sh[1]));
+  // a row of zeros (or of less than the smallest normal scale holds) keeps a finite reciprocal; a NaN stays one (the comparison is false)
+  float scale = most * (1.f / 448.f);
+  if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;
+  if (t == 0) a.scale[r] = scale;
+  const float inv = 1.f / scale;
+  uint8_t* q = static_cast<uint8_t*>(a.y) + r * a.dim;
+#pragma unroll
+  for (int c = 0; c < NV; ++c) store_q<V>(q + (t + c * TPR) * V, v[c], inv, a.dim - (t + c * TPR) * V);
+}
+
+struct NormBwd {
+  void* dx;              // [rows, dim]
+  float* part;           // [gridDim.x][dim]: each workgroup's share of dw [nullable]
+  const void* dy;
+  const void* dh;        // [nullable]
+  const void* h;
+  const void* w;         // [nullable]
+  const float* rstd;
+  int64_t rows, dys, dhs, hs;
+  int dim;
+};
+
+// A workgroup takes rows blockIdx.x * RPB, + gridDim.x * RPB, ...: a thread keeps its columns of w and of dw in registers throughout.
+template <class T, class W, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm_bwd(NormBwd a) {
+  constexpr int V = Row<T>::V, RPB = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float sh[2][TPR / 64];
+  __shared__ float join[RPB > 1 ? NV * V * TPR : 1];
+  const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  constexpr bool KEEP = NV * V * TPR <= 16384;      // wider rows read w again for each row (it stays in L2) rather than spill
+  float w[KEEP ? NV : 1][V], dw[NV][V];
+  auto weight = [&](int c, float (&f)[V]) {
+    if (a.w) { load_v<V>(f, static_cast<const W*>(a.w) + (t + c * TPR) * V, a.dim - (t + c * TPR) * V); return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = 1.f;
+  };
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    if (KEEP) weight(c, w[KEEP ? c : 0]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[c][i] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t r = (int64_t)blockIdx.x * RPB + slot; r < a.rows; r += (int64_t)gridDim.x * RPB, turn ^= 1) {
+    const T* dy = static_cast<const T*>(a.dy) + r * a.dys;
+    const T* h = static_cast<const T*>(a.h) + r * a.hs;
+    const float rstd = a.rstd[r];
+    float d[NV][V], n[NV][V], s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      load_v<V>(d[c], dy + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+      load_v<V>(n[c], h + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+    }
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      if (!KEEP) weight(c, w[0]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        n[c][i] *= rstd;
+        dw[c][i] += d[c][i] * n[c][i];
+        d[c][i] *= w[KEEP ? c : 0][i];
+        s += d[c][i] * n[c][i];
+      }
+    }
+    s = row_sum<TPR>(s, sh[turn]) / (float)a.dim;      // two places in turn: one barrier a row
+    if (!a.dx) continue;
+    T* dx = static_cast<T*>(a.dx) + r * a.dim;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[c][i] = rstd * (d[c][i] - n[c][i] * s);
+      if (a.dh) {
+        float f[V];
+        load_v<V>(f, static_cast<const T*>(a.dh) + r * a.dhs + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[c][i] += f[i];
+      }
+      store_v<V>(dx + (t + c * TPR) * V, d[c], a.dim - (t + c * TPR) * V);
+    }
+  }
+  if (!a.part) return;
+  if (RPB > 1) {                               // the workgroup's rows at once, joined in order
+    for (int k = RPB - 1; k > 0; --k) {
+      if (slot == k) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+          for (int i = 0; i < V; ++i) join[(c * V + i) * TPR + t] = dw[c][i];
+      }
+      __syncthreads();
+      if (slot == k - 1) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+          for (int i = 0; i < V; ++i) dw[c][i] += join[(c * V + i) * TPR + t];
+      }
+      __syncthreads();
+    }
+    if (slot > 0) return;
+  }
+  float* part = a.part + (int64_t)blockIdx.x * a.dim;
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+#pragma unroll
+    for (int i = 0; i < V; ++i) if ((t + c * TPR) * V + i < a.dim) part[(t + c * TPR) * V + i] = dw[c][i];
+}
+
+// dw[c] = sum of the workgroups' shares, in a fixed order
+template <class W> __global__ __launch_bounds__(1024) void k_rms_norm_dw(W* __restrict__ dw, const float* __restrict__ part, int parts, int dim) {
+  __shared__ float sh[16][64];
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6, c = blockIdx.x * 64 + x;
+  float s = 0.f;
+  if (c < dim)
+#pragma unroll 4
+    for (int p = y; p < parts; p += 16) s += part[(int64_t)p * dim + c];
+  sh[y][x] = s;
+  __syncthreads();
+  if (y || c >= dim) return;
+  for (int i = 1; i < 16; ++i) s += sh[i][x];
+  dw[c] = (W)s;
+}
+
+// threads a row and chunks a thread: a wave for up to 128 chunks of 16 bytes (no barrier), then 4 waves, then 16
+#define CAGC_ROW_SHAPES(chunks, CALL)      \
+  if (chunks <= 64) { CALL(64, 1); }       \
+  else if (chunks <= 128) { CALL(64, 2); } \
+  else if (chunks <= 256) { CALL(256, 1); } \
+  else if (chunks <= 512) { CALL(256, 2); } \
+  else if (chunks <= 768) { CALL(256, 3); } \
+  else if (chunks <= 1024) { CALL(256, 4); } \
+  else if (chunks <= 2048) { CALL(1024, 2); } \
+  else { CALL(1024, 4); }
+
+constexpr int MOST_CHUNKS = 4096;
+int esize(int dtype) { return dtype == CAGC_F32 ? 4 : 2; }
+bool row_type(int dtype) { return dtype == CAGC_F32 || dtype == CAGC_F16 || dtype == CAGC_BF16; }
+int chunks_of(int64_t dim, int dtype) { return (int)((dim * esize(dtype) + 15) / 16); }
+bool dim_ok(int64_t dim, int dtype) { return dim > 0 && dim * esize(dtype) <= (int64_t)MOST_CHUNKS * 16; }
+
+template <class T, class W, int OUT> int launch_norm(const Norm& a, hipStream_t st, const char* what) {
+  const int chunks = (a.dim + Row<T>::V - 1) / Row<T>::V;
+#define CAGC_CALL(TPR, NV) hipLaunchKernelGGL((k_rms_norm<T, W, TPR, NV, OUT>), dim3((unsigned)((a.rows + (TPR < 256 ? 256 / TPR : 1) - 1) / (TPR < 256 ? 256 / TPR : 1))), dim3(TPR < 256 ? 256 : TPR), 0, st, a)
+  CAGC_ROW_SHAPES(chunks, CAGC_CALL)
+#undef CAGC_CALL
+  return check_launch(what);
+}
+template <int OUT> int launch_norm_as(const Norm& a, int dtype, int wdtype, hipStream_t st, const char* what) {
+  if (dtype == CAGC_F32) return launch_norm<float, float, OUT>(a, st, what);
+  if (dtype == CAGC_F16) return wdtype == CAGC_F32 ? launch_norm<_Float16, float, OUT>(a, st, what) : launch_norm<_Float16, _Float16, OUT>(a, st, what);
+  return wdtype == CAGC_F32 ? launch_norm<__bf16, float, OUT>(a, st, what) : launch_norm<__bf16, __bf16, OUT>(a, st, what);
+}
+
+// workgroups of a backward: each writes dim floats for dw, so few enough that these stay small beside the rows, enough to fill 256 CUs
+int bwd_wgs(int64_t rows, int chunks) {
+  const int rpb = chunks <= 128 ? 4 : 1;
+  const int64_t need = (rows + rpb - 1) / rpb;
+  return (int)(need < 1024 ? need : 1024);
+}
+
+template <class T, class W> int launch_bwd(const NormBwd& a, void* dw, hipStream_t st, const char* what) {
+  const int chunks = (a.dim + Row<T>::V - 1) / Row<T>::V, wgs = bwd_wgs(a.rows, chunks);
+#define CAGC_CALL(TPR, NV) hipLaunchKernelGGL((k_rms_norm_bwd<T, W, TPR, NV>), dim3(wgs), dim3(TPR < 256 ? 256 : TPR), 0, st, a)
+  CAGC_ROW_SHAPES(chunks, CAGC_CALL)
+#undef CAGC_CALL
+  int rc = check_launch(what);
+  if (rc != CAGC_OK || !dw) return rc;
+  hipLaunchKernelGGL((k_rms_norm_dw<W>), dim3((a.dim + 63) / 64), dim3(1024), 0, st, static_cast<W*>(dw), a.part, wgs, a.dim);
+  return check_launch(what);
+}
+
+}  // namespace
+}  // namespace cagc
+
+using namespace cagc;
+
+#define CAGC_NORM_CHECKS(what)                                                                                                          \
+  CAGC_REQUIRE(row_type(dtype), "%s: element type %d", what, dtype);                                                                    \
+  CAGC_REQUIRE(wdtype == dtype || wdtype == CAGC_F32, "%s: weight type %d for element type %d", what, wdtype, dtype);                   \
+  CAGC_REQUIRE(rows >= 0 && rows < (1ll << 31) && dim_ok(dim, dtype), "%s: %lld rows of %lld (at most %d bytes a row)", what, (long long)rows, (long long)dim, MOST_CHUNKS * 16)
+
+extern "C" int cagc_rms_norm_fwd(void* y, void* h, float* rstd, const void* x, const void* residual, const void* w, int64_t rows, int64_t dim, int64_t x_stride,
+                                 int64_t res_stride, int dtype, int wdtype, float eps, cagc_stream_t stream) {
+  const char* what = "cagc_rms_norm_fwd";
+  CAGC_NORM_CHECKS(what);
+  if (rows == 0) return CAGC_OK;
+  CAGC_REQUIRE(y && x && (!residual || h), "%s: null pointer", what);
+  const Norm a = {y, nullptr, h, rstd, x, residual, w, rows, x_stride, res_stride, (int)dim, eps};
+  return launch_norm_as<0>(a, dtype, wdtype, as_stream(stream), what);
+}
+extern "C" int cagc_rms_norm_e4m3(void* q, float* scale, void* h, const void* x, const void* residual, const void* w, int64_t rows, int64_t dim, int64_t x_stride,
+                                  int64_t res_stride, int dtype, int wdtype, float eps, cagc_stream_t stream) {
+  const char* what = "cagc_rms_norm_e4m3";
+  CAGC_NORM_CHECKS(what);
+  if (rows == 0) return CAGC_OK;
+  CAGC_REQUIRE(q && scale && x && (!residual || h), "%s: null pointer", what);
+  const Norm a = {q, scale, h, nullptr, x, residual, w, rows, x_stride, res_stride, (int)dim, eps};
+  return launch_norm_as<1>(a, dtype, wdtype, as_stream(stream), what);
+}
+extern "C" int cagc_quantize_rows_e4m3(void* q, float* scale, const void* x, int64_t rows, int64_t dim, int64_t x_stride, int dtype, cagc_stream_t stream) {
+  const char* what = "cagc_quantize_rows_e4m3";
+  const int wdtype = dtype;
+  CAGC_NORM_CHECKS(what);
+  if (rows == 0) return CAGC_OK;
+  CAGC_REQUIRE(q && scale && x, "%s: null pointer", what);
+  const Norm a = {q, scale, nullptr, nullptr, x, nullptr, nullptr, rows, x_stride, 0, (int)dim, 0.f};
+  return launch_norm_as<2>(a, dtype, dtype, as_stream(stream), what);
+}
+extern "C" int64_t cagc_rms_norm_bwd_workspace(int64_t rows, int64_t dim, int dtype) {
+  if (rows <= 0 || !row_type(dtype) || !dim_ok(dim, dtype)) return 0;
+  return 4 * dim * bwd_wgs(rows, chunks_of(dim, dtype));
+}
+extern "C" int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, const void* dh, const void* h, const void* w, const float* rstd, int64_t rows,
+                                 int64_t dim, int64_t dy_stride, int64_t dh_stride, int64_t h_stride, int dtype, int wdtype, cagc_stream_t stream) {
+  const char* what = "cagc_rms_norm_bwd";
+  CAGC_NORM_CHECKS(what);
+  CAGC_REQUIRE(rows > 0, "%s: no rows (the weight's gradient is zero)", what);
+  if (!dx && !dw) return CAGC_OK;
+  CAGC_REQUIRE(dy && h && rstd && (!dw || ws), "%s: null pointer", what);
+  const NormBwd a = {dx, dw ? static_cast<float*>(ws) : nullptr, dy, dh, h, w, rstd, rows, dy_stride, dh_stride, h_stride, (int)dim};
+  hipStream_t st = as_stream(stream);
+  if (dtype == CAGC_F32) return launch_bwd<float, float>(a, dw, st, what);
+  if (dtype == CAGC_F16) return wdtype == CAGC_F32 ? launch_bwd<_Float16, float>(a, dw, st, what) : launch_bwd<_Float16, _Float16>(a, dw, st, what);
+  return wdtype == CAGC_F32 ? launch_bwd<__bf16, float>(a, dw, st, what) : launch_bwd<__bf16, __bf16>(a, dw, st, what);
+}

@@ -71,6 +71,12 @@ typedef void* cagc_stream_t; /* hipStream_t */
 #define CAGC_F32 0
 #define CAGC_F16 1
 #define CAGC_F64 2
+/* further element types of the row-wise and gated operators (cagc_rms_norm_*, cagc_gated_linear_*, cagc_grad_*) */
+#define CAGC_BF16 3
+#define CAGC_E4M3 4   /* 8-bit float, 4 exponent and 3 mantissa bits, no infinities (OCP e4m3fn) */
+/* activations of cagc_gated_linear_* */
+#define CAGC_ACT_SILU 0
+#define CAGC_ACT_GELU 1   /* g Phi(g), by the error function */
 
 int cagc_abi_version(void);
 const char* cagc_last_error(void);
@@ -523,6 +529,55 @@ int cagc_to_phase_planar(float* t, const float* x, int64_t planes, int H, int W,
 
 /* out[i] = (a[i] + b[i]) * scale — ResBlock merge (conv path + skip) / sqrt(2) (model.py:736) in one pass. */
 int cagc_add_scale(float* out, const float* a, const float* b, int64_t n, float scale, cagc_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * root-mean-square norm of rows:  h = x + residual (rounded to the type; h = x without a residual),
+ *     rstd = (mean(h^2) + eps)^-1/2,  y = h * rstd * w
+ * x, residual [nullable]: rows x_stride / res_stride elements apart, any alignment; y and h contiguous; h is required with a residual, otherwise nullable;
+ * w [dim] [nullable] in wdtype = dtype or CAGC_F32; rstd [rows] [nullable] is what the backward pass reads.  dtype: CAGC_F32 / F16 / BF16, sums in fp32.
+ * rows 0 is a no-op; a row holds at most 64 KiB.
+ * ---------------------------------------------------------------------------------------------- */
+int cagc_rms_norm_fwd(void* y, void* h, float* rstd, const void* x, const void* residual, const void* w, int64_t rows, int64_t dim, int64_t x_stride,
+                      int64_t res_stride, int dtype, int wdtype, float eps, cagc_stream_t stream);
+/* the same with y in 8 bits: scale[row] = max(max |y| / 448, 2^-126), q = y / scale rounded to e4m3 (a row with a NaN has a NaN scale) */
+int cagc_rms_norm_e4m3(void* q, float* scale, void* h, const void* x, const void* residual, const void* w, int64_t rows, int64_t dim, int64_t x_stride,
+                       int64_t res_stride, int dtype, int wdtype, float eps, cagc_stream_t stream);
+/* rows as they are -> e4m3 and a scale per row (weights, once) */
+int cagc_quantize_rows_e4m3(void* q, float* scale, const void* x, int64_t rows, int64_t dim, int64_t x_stride, int dtype, cagc_stream_t stream);
+/* dx [rows, dim] (contiguous; also the residual's gradient) and dw [dim] in wdtype, each nullable; dh [nullable]: the gradient of h from its other use;
+ * dy, dh, h: rows dy_stride, dh_stride, h_stride apart.  rows > 0.  ws: cagc_rms_norm_bwd_workspace bytes (only with dw).  Fixed order of summation. */
+int64_t cagc_rms_norm_bwd_workspace(int64_t rows, int64_t dim, int dtype);
+int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, const void* dh, const void* h, const void* w, const float* rstd, int64_t rows,
+                      int64_t dim, int64_t dy_stride, int64_t dh_stride, int64_t h_stride, int dtype, int wdtype, cagc_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * gated projection:   out[m][j] = act(s * sum_k x[m][k] w[j][k] + bias[j]) * (s * sum_k x[m][k] w[n+j][k] + bias[n+j])
+ * w is [2n, k]: the n gate rows, then the n up rows.  x [rows, k] and w may have rows further apart than k (ldx, ldw: elements);
+ * out [rows, n] is contiguous.  dtype: CAGC_F32 / F16 / BF16, sums in fp32, one rounding to out_dtype (= dtype).
+ * dtype CAGC_E4M3: x and w hold e4m3 values, x_scale [rows] and w_scale [2n] multiply their rows; out_dtype F32 / F16 / BF16, bias in
+ * that type.  Any k, n, alignment; rows 0 is a no-op.  Rows (k) up to 7 MiB.
+ * saved [nullable]: pre-activations for the backward pass: fp32 [2][rows][n]; 16-bit types: uint16 [3][rows][n] (24 bits of each).
+ * ws: cagc_gated_linear_workspace bytes (0: may be null), 256-byte aligned.
+ * ---------------------------------------------------------------------------------------------- */
+int64_t cagc_gated_linear_workspace(const void* x, const void* w, int64_t rows, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int dtype);
+int cagc_gated_linear_fwd(void* out, void* saved /*[nullable]*/, void* ws, const void* x, const void* w, const void* bias /*[nullable]*/,
+                          const float* x_scale /*[nullable]*/, const float* w_scale /*[nullable]*/, int64_t rows, int64_t n, int64_t k,
+                          int64_t ldx, int64_t ldw, int dtype, int out_dtype, int act, float scale, cagc_stream_t stream);
+/* dx [rows, k], dw [2n, k], db [2n] (each nullable: not wanted), contiguous, in dtype; dy [rows, n] with rows lddy apart.  rows > 0.  Every sum runs in
+ * a fixed order: two calls give the same bits. */
+int64_t cagc_gated_linear_bwd_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int need_dx, int need_dw, int need_db);
+int cagc_gated_linear_bwd(void* dx, void* dw, void* db, void* ws, const void* dy, const void* saved, const void* x, const void* w, int64_t rows,
+                          int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t lddy, int dtype, int act, float scale, cagc_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * norm over `count` contiguous tensors together (host arrays p, n: elements, dtype: CAGC_F32 / F16 / BF16 each), norm_type 1, 2 or 0 (largest magnitude), and,
+ * with scale != 0, the tensors times min(1, max_norm / (norm + 1e-6)) in place.  *norm (device) gets the norm in fp32; sums run in 64 bits, in a fixed order.
+ * A NaN or infinity shows in the norm, and a NaN norm makes the scaled tensors NaN.  Tensors that share memory are refused.
+ * ws: cagc_grad_norm_workspace bytes, 64-byte aligned.  The host arrays may be freed after the call (also under stream capture).
+ * ---------------------------------------------------------------------------------------------- */
+int64_t cagc_grad_norm_workspace(const int64_t* n, int count);
+int cagc_clip_grad_norm(float* norm, void* ws, void* const* p, const int64_t* n, const int* dtype, int count, int norm_type, double max_norm, int scale,
+                        cagc_stream_t stream);
 
 #ifdef __cplusplus
 }

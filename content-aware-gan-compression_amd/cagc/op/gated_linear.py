@@ -79,7 +79,7 @@ class _GatedLinear(Function):
         db = torch.empty(2 * n, dtype=dt, device=dev) if want_b else None
         code = _lib.ROW_DTYPE[dt]
         with _lib.on_device(x):
-            need = _lib.query("cagc_gated_linear_bwd_workspace", rows, n, k, code, want_x, want_w, want_b)
+            need = _lib.query("cagc_gated_linear_bwd_workspace", x.data_ptr(), w.data_ptr(), rows, n, k, ldx, ldw, code, want_x, want_w, want_b)
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
             _lib.call("cagc_gated_linear_bwd", _p(dx), _p(dw), _p(db), ws.data_ptr(), g.data_ptr(), saved.data_ptr(), x.data_ptr(), w.data_ptr(), rows, n, k,
                       ldx, ldw, ldg, code, ctx.act, ctx.scale)

@@ -1,6 +1,6 @@
 // Shared pieces of the gated projection (gated.hip): element types, the activation, the saved pre-activations.
 #pragma once
-#include "common.h"
+#include "rows.h"
 
 namespace cagc {
 namespace gated {
@@ -45,9 +45,18 @@ template <> __device__ __forceinline__ f32x4 mma<e4m3>(const i32x4 (&a)[2], cons
 }
 
 // act(g) and act'(g).  SiLU: g s with s = 1 / (1 + e^-g), derivative s (1 + g (1 - s)); GELU: g Phi(g), derivative Phi(g) + g phi(g).
+// Phi by Abramowitz and Stegun's formula 7.1.26 (erf to 1.5e-7, so Phi to 0.8e-7, little over an fp32 rounding of 1): without branches, and its exponential is phi's
+// too.  The library's erff takes both sides of a branch in a wave that holds values of either size.
+__device__ __forceinline__ float normal_cdf(float g, float& e) {
+  const float x = fabsf(g) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+  e = __expf(-0.5f * g * g);
+  const float poly = ((((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f) * t, half = 0.5f * poly * e;
+  return g < 0.f ? half : 1.f - half;
+}
 __device__ __forceinline__ float act_of(int act, float g) {
   if (act == CAGC_ACT_SILU) return g * __builtin_amdgcn_rcpf(1.f + __expf(-g));
-  return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+  float e;
+  return g * normal_cdf(g, e);
 }
 __device__ __forceinline__ void act_grad(int act, float g, float& a, float& da) {
   if (act == CAGC_ACT_SILU) {
@@ -56,20 +65,24 @@ __device__ __forceinline__ void act_grad(int act, float g, float& a, float& da) 
     da = s * (1.f + g * (1.f - s));
     return;
   }
-  const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+  float e;
+  const float c = normal_cdf(g, e);
   a = g * c;
-  da = c + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
+  da = c + g * e * 0.39894228040143268f;
 }
 
-// Saved pre-activations.  fp32: two planes [rows, n].  16-bit types: the upper 24 bits of each fp32 value, as three 16-bit planes (the
-// upper halves of g, of u, and the two third bytes).  Rounding them to the input's type instead (2 planes) would add an error as
-// large as that of the gradients' own rounding: measured against 64 bits, the gradients' error in bf16 is 1.4 times that of one
-// final rounding with 24 bits and 1.8 times with 16.
-__device__ __forceinline__ uint32_t top24(float v) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, v);
-  return (b & 0x7fffffffu) > 0x7f800000u ? 0x7fc000u : (b + 0x80u) >> 8;
-}
+// Saved pre-activations.  fp32: two planes [rows, n].  16-bit types: the upper 24 bits of each fp32 value (a significand of 16 bits, cut: within 2^-15 of the value, and a
+// NaN's quiet bit stays), as three 16-bit planes: the upper halves of g, of u, and their third bytes (g's in the upper byte).  Rounding them to the input's
+// type instead (2 planes) would add an error as large as that of the gradients' own rounding: against 64 bits, the gradients' error in bf16 is 1.4 times
+// that of one final rounding with 24 bits and 1.8 times with 16.
 __device__ __forceinline__ float from24(uint32_t hi, uint32_t lo) { return __builtin_bit_cast(float, (hi << 16) | (lo << 8)); }
+__device__ __forceinline__ uint32_t bits(float v) { return __builtin_bit_cast(uint32_t, v); }
+// the upper halves of two values; the third bytes of two values each of g and u
+__device__ __forceinline__ uint32_t upper2(float a, float b) { return __builtin_amdgcn_perm(bits(b), bits(a), 0x07060302u); }
+__device__ __forceinline__ uint32_t third2(float g0, float u0, float g1, float u1) {
+  const uint32_t x = __builtin_amdgcn_perm(bits(g0), bits(u0), 0x0c0c0501u), y = __builtin_amdgcn_perm(bits(g1), bits(u1), 0x0c0c0501u);
+  return x | y << 16;
+}
 
 }  // namespace gated
 }  // namespace cagc

@@ -5,6 +5,7 @@
 // pre-activations never travel (a training forward stores them once, for the backward).  Backward, with z = (g, u):
 // dz = (dy u act'(g), dy act(g)) [rows, 2n], dx = s dz W, dW = s dz^T x, db = sum of dz's rows.
 #include "gated.h"
+#include <type_traits>
 
 namespace cagc {
 namespace gated {
@@ -13,12 +14,14 @@ namespace {
 enum { EPI_GATED = 0, EPI_PLAIN = 1 };
 
 struct Product {
-  const char* p;         // operand of the output's columns: [rows, K], rows ldp bytes apart (gated: gate rows, then up rows from p2)
+  const char* p;         // operand of the output's columns (gated: gate rows, then up rows from p2)
   const char* p2;
   const char* q;         // operand of the output's rows
-  int64_t ldp, ldq;
+  int64_t ldp, ldq;      // bytes from row to row
   int np, nq;            // columns and rows of the output
-  int kbytes, ksteps;    // K in bytes and in steps of 128 bytes
+  int kbytes;            // K in bytes (a multiple of 16) where a row holds K ...
+  int krows;             // ... and in rows where a column does
+  int ksteps;            // K in stages
   int splits;            // K is cut into this many pieces, each with a slab of its own
   int tiles_p, tiles_q;
   float* slab;           // [splits][nq][np or 2 np] fp32
@@ -33,101 +36,103 @@ struct Product {
 };
 
 typedef __attribute__((address_space(3))) char lds_t;
-
-template <class T> __device__ __forceinline__ void store4(T* p, f32x4 v, int n, bool vec) {
-  typedef T tx4 __attribute__((ext_vector_type(4)));
-  if (vec && n >= 4) { *reinterpret_cast<tx4*>(p) = tx4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}; return; }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) if (r < n) p[r] = (T)v[r];
-}
-// the gated epilogue for the (up to) four outputs [m][n .. n+3]
-template <class O> __device__ __forceinline__ void gated_out(const Product& a, int m, int n, f32x4 g, f32x4 u) {
-  const int left = a.np - n;
-  const float sq = a.alpha * (a.sq ? a.sq[m] : 1.f);
-  f32x4 o;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    if (r >= left) { g[r] = u[r] = o[r] = 0.f; continue; }
-    g[r] *= a.sp ? sq * a.sp[n + r] : sq;
-    u[r] *= a.sp ? sq * a.sp[a.np + n + r] : sq;
-    if (a.bias) {
-      g[r] += (float)static_cast<const O*>(a.bias)[n + r];
-      u[r] += (float)static_cast<const O*>(a.bias)[a.np + n + r];
-    }
-    o[r] = act_of(a.act, g[r]) * u[r];
-  }
-  const bool vec = (a.np & 3) == 0;
-  const int64_t at = (int64_t)m * a.ldo + n;
-  store4(static_cast<O*>(a.out) + at, o, left, vec);
-  if (!a.saved) return;
-  const int64_t plane = (int64_t)a.nq * a.np, i = (int64_t)m * a.np + n;
-  if (sizeof(O) == 4) {
-    store4(static_cast<float*>(a.saved) + i, g, left, vec);
-    store4(static_cast<float*>(a.saved) + plane + i, u, left, vec);
-    return;
-  }
-  typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
-  u16x4 hg, hu, lo;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const uint32_t tg = top24(g[r]), tu = top24(u[r]);
-    hg[r] = (uint16_t)(tg >> 8); hu[r] = (uint16_t)(tu >> 8); lo[r] = (uint16_t)((tg & 0xffu) << 8 | (tu & 0xffu));
-  }
-  uint16_t* s = static_cast<uint16_t*>(a.saved) + i;
-  if (vec && left >= 4) {
-    *reinterpret_cast<u16x4*>(s) = hg; *reinterpret_cast<u16x4*>(s + plane) = hu; *reinterpret_cast<u16x4*>(s + 2 * plane) = lo;
-    return;
-  }
-  for (int r = 0; r < 4; ++r) if (r < left) { s[r] = hg[r]; s[plane + r] = hu[r]; s[2 * plane + r] = lo[r]; }
-}
-template <class O> __device__ __forceinline__ void plain_out(const Product& a, int m, int n, f32x4 v) {
-  store4(static_cast<O*>(a.out) + (int64_t)m * a.ldo + n, v * a.alpha, a.np - n, (a.ldo & 3) == 0);
-}
+template <class V> __device__ __forceinline__ V lds_read(const lds_t* p) { return *reinterpret_cast<const __attribute__((address_space(3))) V*>(p); }
 
 // ---- tiled product --------------------------------------------------------------------------------------------------------------
 // out[m][n] = sum_k q[m][k] p[n][k].  A workgroup of WP x WQ waves makes a tile of BQ rows (m) and BP rows of p (n; gated: BP/2 columns,
 // gate and up); K goes by in stages of 128 bytes a row, two stages in LDS: while one is multiplied, the other is filled by loads that
-// go straight to LDS.  A stage's row is 8 chunks of 16 bytes, chunk c kept at slot c ^ (row % 8): the 16 rows that a wave reads of one
-// chunk then lie in different banks; the loads write LDS in lane order, so the lanes fetch their chunks in that order.
-// Rows beyond the operand are read from its last row (their outputs are not stored), chunks beyond K come back as zero.
-template <class T, class O, int BP, int BQ, int WP, int WQ, int EPI> struct Tile {      // (O: a class of its own for each kernel)
-  static constexpr int NW = WP * WQ, TP = BP / WP, TQ = BQ / WQ, IP = TP / 16, IQ = TQ / 16;
-  static constexpr int LOADS = (BP + BQ) / 8 / NW;                 // direct loads of a wave and stage, 8 rows each
-  static constexpr int STAGE = (BP + BQ) * 128;
-  static_assert((BP / 16) % NW == 0 && (BQ / 8) % NW == 0, "a load's 8 rows lie in one operand");
-  f32x4 acc[IP][IQ];
-
-  __device__ __forceinline__ void step(lds_t* __restrict__ cur, lds_t* __restrict__ nxt, const __amdgpu_buffer_rsrc_t (&rs)[3],
-                                       const int (&off)[LOADS], int next, bool more, bool tail_ok, int w, int pa, int qa, int c0, int c1) {
-    if (more) fill(nxt, rs, off, next, tail_ok, w);
-    {
-      i32x4 pf[IP][2], qf[IQ][2];
+// go straight to LDS, in lane order, 16 bytes a lane.
+//
+// An operand lies in memory with K along its rows (x, W in the forward), or with K down its columns (W for dx; dz and x for dW).  In LDS a stage keeps that
+// order: B rows of 128 bytes, or 128 / size rows of B elements.  Along rows, a wave reads 16 bytes of 16 rows at a time; down columns, the
+// transposing read hands each lane 4 elements of a column (16-bit types), or it reads single elements (fp32).  Either way a lane ends up with the k that the other operand's lane
+// has: chunk number lane / 16 (and 4 + lane / 16) of the stage's eight.  So that those reads fall into different banks, chunk c of LDS row r is kept at c ^ turn(r).
+// Nothing outside the operands is read: rows beyond the last repeat it (their outputs are not stored), chunks beyond a row and rows beyond K come back as zero.
+template <class T, int B, bool DOWN> struct Side {
+  static constexpr int ES = Type<T>::size, RK = 128 / ES;          // elements of K in a stage
+  static constexpr int ROW = DOWN ? B * ES : 128, CH = ROW / 16;   // bytes and chunks of an LDS row
+  static __device__ __forceinline__ int turn(int row) {
+    if (!DOWN) return row & 7;
+    if (ES == 2) return (((row & 3) | ((row >> 3) & 1) << 2) << 1) & (CH - 1);
+    return (((row >> 2) & 3) << 2) & (CH - 1);
+  }
+  // where the 16 bytes at `at` of the stage come from, as an offset from the tile's first element of the stage.  Along rows: beyond the last row, that row.
+  // Down columns: `columns` bytes are left of a row; a chunk beyond them is out of range for good.
+  static __device__ __forceinline__ int source(int at, int64_t ld, int last, int columns) {
+    const int row = at / ROW, chunk = ((at % ROW) / 16) ^ turn(row);
+    if (!DOWN) return min(row, last) * (int)ld + chunk * 16;
+    return chunk * 16 < columns ? row * (int)ld + chunk * 16 : (int)0x80000000;
+  }
+  // Load number c of a wave of NW begins c * NW KB behind load 0: the same chunk of later rows (along rows), a later row of K (down columns).  What decides whether a
+  // load lies within K is `first` = its chunk's byte or its row of K for c = 0, and c times this:
+  template <int NW> static constexpr int further() { return DOWN ? NW * 1024 / ROW : 0; }
+  static __device__ __forceinline__ int first(int at) { return DOWN ? at / ROW : (((at % ROW) / 16) ^ turn(at / ROW)) * 16; }
+  // LDS address of this lane's part of the 16 columns / rows `t` (in sixteens)
+  static __device__ __forceinline__ int place(int t, int lane) {
+    const int g = lane >> 4, l = lane & 15;
+    if (!DOWN) return (t * 16 + l) * 128;
+    if (ES == 2) { const int row = 8 * g + (l >> 2); return row * ROW + (((2 * t) ^ turn(row)) + ((l & 3) >> 1)) * 16 + (l & 1) * 8; }
+    const int row = 4 * g;
+    return row * ROW + (((4 * t) ^ turn(row)) + (l >> 2)) * 16 + (l & 3) * 4;
+  }
+  static __device__ __forceinline__ i32x4 read(const lds_t* stage, int at, int half, int c) {
+    if (!DOWN) return lds_read<i32x4>(stage + at + c);
+    if constexpr (ES == 2) {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4* tr_t;
+      union { s16x4 h[2]; i32x4 v; } u;
+      u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)(stage + at + half * 32 * ROW));
+      u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)(stage + at + half * 32 * ROW + 4 * ROW));
+      return u.v;
+    } else {
+      i32x4 v;
 #pragma unroll
-      for (int i = 0; i < IP; ++i) {
-        const int row = EPI == EPI_GATED && i >= IP / 2 ? pa + BP / 2 * 128 + (i - IP / 2) * 2048 : pa + i * 2048;
-        pf[i][0] = *reinterpret_cast<__attribute__((address_space(3))) i32x4*>(cur + row + c0);
-        pf[i][1] = *reinterpret_cast<__attribute__((address_space(3))) i32x4*>(cur + row + c1);
-      }
-#pragma unroll
-      for (int j = 0; j < IQ; ++j) {
-        qf[j][0] = *reinterpret_cast<__attribute__((address_space(3))) i32x4*>(cur + qa + j * 2048 + c0);
-        qf[j][1] = *reinterpret_cast<__attribute__((address_space(3))) i32x4*>(cur + qa + j * 2048 + c1);
-      }
-#pragma unroll
-      for (int j = 0; j < IQ; ++j)
-#pragma unroll
-        for (int i = 0; i < IP; ++i) acc[i][j] = mma<T>(pf[i], qf[j], acc[i][j]);
+      for (int j = 0; j < 4; ++j) v[j] = lds_read<int>(stage + at + (half * 16 + j) * ROW);
+      return v;
     }
   }
-  // the loads of a stage: number c of this wave fills the 8 rows from (c * NW + w) * 8
-  static __device__ __forceinline__ void fill(lds_t* __restrict__ dst, const __amdgpu_buffer_rsrc_t (&rs)[3], const int (&off)[LOADS], int step,
-                                              bool ok, int w) {
+};
+
+template <class T, class O, int BP, int BQ, int WP, int WQ, int EPI, bool DP, bool DQ> struct Tile {      // (O: a class of its own for each kernel)
+  typedef Side<T, BP, DP> P;
+  typedef Side<T, BQ, DQ> Q;
+  static constexpr int NW = WP * WQ, TP = BP / WP, TQ = BQ / WQ, IP = TP / 16, IQ = TQ / 16;
+  static constexpr int LP = BP / 8 / NW, LQ = BQ / 8 / NW;         // loads of 1 KB of a wave and stage
+  static constexpr int STAGE = (BP + BQ) * 128;
+  static_assert(BP % (16 * NW) == 0 && BQ % (8 * NW) == 0, "a wave's loads lie in one operand, and in one half of p");
+  f32x4 acc[IP][IQ];
+  int pa[IP], qa[IQ];              // LDS places of this lane's operands
+  int po[LP], qo[LQ];              // sources of this lane's loads
+  int pk, qk;                      // Side::first of them
+
+  __device__ __forceinline__ void fill(lds_t* __restrict__ dst, const Product& a, const char* p, const char* p2, const char* q, int step, int w) {
+    const int pl = DP ? a.krows - step * P::RK : a.kbytes - step * 128, ql = DQ ? a.krows - step * Q::RK : a.kbytes - step * 128;      // what is left of K
 #pragma unroll
-    for (int c = 0; c < LOADS; ++c) {
-      const int first = c * NW * 8;
-      const __amdgpu_buffer_rsrc_t r = first < BP / 2 ? rs[0] : (first < BP ? rs[1] : rs[2]);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + (first + w * 8) * 128), 16,
-                                               ok ? off[c] : (int)0x80000000, step * 128, 0, 0);
+    for (int c = 0; c < LP; ++c) {
+      const int at = c * NW * 1024;
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(!DP && at >= BP * 64 ? p2 : p), 0, 0x7ffffff0, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + at + w * 1024), 16,
+                                               pk + c * P::template further<NW>() < pl ? po[c] : (int)0x80000000, 0, 0, 0);
+    }
+#pragma unroll
+    for (int c = 0; c < LQ; ++c) {
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)q, 0, 0x7ffffff0, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + BP * 128 + c * NW * 1024 + w * 1024), 16,
+                                               qk + c * Q::template further<NW>() < ql ? qo[c] : (int)0x80000000, 0, 0, 0);
+    }
+  }
+  // (one function with both stages as restricted pointers: the compiler then knows that the loads into `nxt` do not touch what is read from `cur`, and does not wait for them)
+  __device__ __forceinline__ void step(lds_t* __restrict__ cur, lds_t* __restrict__ nxt, const Product& a, const char* p, const char* p2, const char* q, int next, bool more, int w,
+                                       int c0, int c1) {
+    if (more) fill(nxt, a, p, p2, q, next, w);
+    i32x4 pf[IP][2];
+#pragma unroll
+    for (int i = 0; i < IP; ++i) { pf[i][0] = P::read(cur, pa[i], 0, c0); pf[i][1] = P::read(cur, pa[i], 1, c1); }
+#pragma unroll
+    for (int j = 0; j < IQ; ++j) {
+      const i32x4 qf[2] = {Q::read(cur + BP * 128, qa[j], 0, c0), Q::read(cur + BP * 128, qa[j], 1, c1)};
+#pragma unroll
+      for (int i = 0; i < IP; ++i) acc[i][j] = mma<T>(pf[i], qf, acc[i][j]);
     }
   }
 };
@@ -143,77 +148,243 @@ __device__ __forceinline__ void tile_of(int b, int tiles_p, int tiles_q, int& tp
   tp = in / rows;
 }
 
-template <class T, class O, int BP, int BQ, int WP, int WQ, int EPI>
+// A tile's results leave through LDS, so that whole rows of the tile are written at once (a lane holds 4 columns of one row; stores of its 8 bytes, 32 contiguous
+// bytes a row, took three times as long).  ROWS x COLS elements of type E at `lds`, chunk c of row r at c ^ (r % 16).
+template <class E, int ROWS, int COLS, int NT> struct Out {
+  static constexpr int ROW = COLS * (int)sizeof(E), CH = ROW / 16, BYTES = ROWS * ROW;
+  typedef E e4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ void put(lds_t* lds, int row, int col, e4 v) {
+    const int byte = col * (int)sizeof(E);
+    *reinterpret_cast<__attribute__((address_space(3))) e4*>(lds + row * ROW + (((byte / 16) ^ (row & (CH < 16 ? CH - 1 : 15))) * 16) + byte % 16) = v;
+  }
+  static __device__ __forceinline__ void store(const lds_t* lds, E* base, int64_t ld, int rows, int cols) {
+#pragma unroll
+    for (int c = 0; c < (ROWS * CH + NT - 1) / NT; ++c) {
+      const int id = c * NT + threadIdx.x, row = id / CH, chunk = id % CH, col = chunk * (16 / (int)sizeof(E));
+      if (ROWS * CH % NT && id >= ROWS * CH) return;
+      if (row >= rows || col >= cols) continue;
+      const i32x4 v = lds_read<i32x4>(lds + row * ROW + ((chunk ^ (row & (CH < 16 ? CH - 1 : 15))) * 16));
+      E* to = base + (int64_t)row * ld + col;
+      if (col + 16 / (int)sizeof(E) <= cols) *reinterpret_cast<Any16*>(to) = __builtin_bit_cast(Any16, v);
+      else {
+        union { i32x4 v; E e[16 / sizeof(E)]; } u;
+        u.v = v;
+#pragma unroll
+        for (int i = 0; i < 16 / (int)sizeof(E); ++i) if (i < cols - col) to[i] = u.e[i];
+      }
+    }
+  }
+};
+
+// four values from s[n], those from s[last + 1] on repeating s[last]
+template <class O> __device__ __forceinline__ f32x4 four_of(const O* s, int n, int last) {
+  f32x4 b;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) b[r] = (float)s[min(n + r, last)];
+  return b;
+}
+template <int ACT> __device__ __forceinline__ f32x4 gate(f32x4 g, f32x4 u) {
+  f32x4 o;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = act_of(ACT, g[r]) * u[r];
+  return o;
+}
+template <class E> __device__ __forceinline__ void put4(E* p, f32x4 v, int left) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) if (r < left) p[r] = (E)v[r];
+}
+
+template <class T, class O, int BP, int BQ, int WP, int WQ, int EPI, bool DP, bool DQ>
 __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
-  typedef Tile<T, O, BP, BQ, WP, WQ, EPI> K;
+  typedef Tile<T, O, BP, BQ, WP, WQ, EPI, DP, DQ> K;
+  constexpr bool GATED = EPI == EPI_GATED;
+  constexpr int COLS = GATED ? BP / 2 : BP, NT = WP * WQ * 64;
   __shared__ __attribute__((aligned(1024))) char stage[2 * K::STAGE];
   lds_t* s0 = (lds_t*)stage;
   lds_t* s1 = s0 + K::STAGE;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = w % WP, wq = w / WP;
   int tp, tq;
   tile_of(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
-  constexpr int COLS = EPI == EPI_GATED ? BP / 2 : BP;
   const int n0 = tp * COLS, m0 = tq * BQ;
-  // this split's K steps
-  const int per = (a.ksteps + a.splits - 1) / a.splits, k0 = blockIdx.y * per, k1 = min(a.ksteps, k0 + per);
-
-  __amdgpu_buffer_rsrc_t rs[3];
-  const int lp0 = EPI == EPI_GATED ? n0 : n0 + BP / 2;
-  const char* second = EPI == EPI_GATED ? a.p2 : a.p;
-  rs[0] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p + (int64_t)min(n0, a.np - 1) * a.ldp), 0, 0x7ffffff0, 0x00020000);
-  rs[1] = __builtin_amdgcn_make_buffer_rsrc((void*)(second + (int64_t)min(lp0, a.np - 1) * a.ldp), 0, 0x7ffffff0, 0x00020000);
-  rs[2] = __builtin_amdgcn_make_buffer_rsrc((void*)(a.q + (int64_t)m0 * a.ldq), 0, 0x7ffffff0, 0x00020000);
-  const int chunk = (lane & 7) ^ (lane >> 3);
-  int off[K::LOADS];
-#pragma unroll
-  for (int c = 0; c < K::LOADS; ++c) {
-    const int row = (c * K::NW + w) * 8 + (lane >> 3);
-    const int first = c * K::NW * 8;
-    if (first < BP / 2) off[c] = min(row, max(0, a.np - 1 - n0)) * (int)a.ldp;
-    else if (first < BP) off[c] = min(row - BP / 2, max(0, a.np - 1 - lp0)) * (int)a.ldp;
-    else off[c] = min(row - BP, a.nq - 1 - m0) * (int)a.ldq;
-    off[c] += chunk * 16;
-  }
-  const int pa = (wp * (EPI == EPI_GATED ? K::TP / 2 : K::TP) + (lane & 15)) * 128, qa = (BP + wq * K::TQ + (lane & 15)) * 128;
-  const int c0 = ((lane >> 4) ^ (lane & 7)) * 16, c1 = ((4 + (lane >> 4)) ^ (lane & 7)) * 16;
-  auto inside = [&](int step) { return step * 128 + chunk * 16 < a.kbytes; };
+  const int per = (a.ksteps + a.splits - 1) / a.splits, k0 = blockIdx.y * per, k1 = min(a.ksteps, k0 + per);      // this split's stages
 
   K t;
+  // first elements of the tile's operands at stage k0, and how far a stage moves them
+  const int64_t dp = DP ? K::P::RK * a.ldp : 128, dq = DQ ? K::Q::RK * a.ldq : 128;
+  const int second = min(n0 + BP / 2, a.np - 1);      // (not gated, K along rows: the tile's other half of rows)
+  const char* p = a.p + (DP ? (int64_t)n0 * K::P::ES : (int64_t)n0 * a.ldp) + k0 * dp;
+  const char* p2 = (GATED ? a.p2 + (int64_t)n0 * a.ldp : a.p + (int64_t)second * a.ldp) + k0 * dp;
+  const char* q = a.q + (DQ ? (int64_t)m0 * K::Q::ES : (int64_t)m0 * a.ldq) + k0 * dq;
+  const int mine = w * 1024 + lane * 16;
+  t.pk = K::P::first(mine);
+  t.qk = K::Q::first(mine);
+#pragma unroll
+  for (int c = 0; c < K::LP; ++c) {
+    const int at = c * K::NW * 1024 + mine;
+    const bool upper = !DP && c * K::NW * 1024 >= BP * 64;
+    t.po[c] = K::P::source(upper ? at - BP * 64 : at, a.ldp, a.np - 1 - (upper && !GATED ? second : n0), (a.np - n0) * K::P::ES);
+  }
+#pragma unroll
+  for (int c = 0; c < K::LQ; ++c) t.qo[c] = K::Q::source(c * K::NW * 1024 + mine, a.ldq, a.nq - 1 - m0, (a.nq - m0) * K::Q::ES);
+#pragma unroll
+  for (int i = 0; i < K::IP; ++i)
+    t.pa[i] = K::P::place(GATED ? (i < K::IP / 2 ? wp * (K::IP / 2) + i : BP / 32 + wp * (K::IP / 2) + i - K::IP / 2) : wp * K::IP + i, lane);
+#pragma unroll
+  for (int j = 0; j < K::IQ; ++j) t.qa[j] = K::Q::place(wq * K::IQ + j, lane);
+  const int c0 = ((lane >> 4) ^ (lane & 7)) * 16, c1 = ((4 + (lane >> 4)) ^ (lane & 7)) * 16;
 #pragma unroll
   for (int i = 0; i < K::IP; ++i)
 #pragma unroll
     for (int j = 0; j < K::IQ; ++j) t.acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (k0 < k1) K::fill(s0, rs, off, k0, inside(k0), w);
+
+  if (k0 < k1) t.fill(s0, a, p, p2, q, k0, w);
   for (int k = k0; k < k1; ++k) {
+    p += dp; p2 += dp; q += dq;
     __builtin_amdgcn_s_waitcnt(0x0f70);      // this wave's loads have reached LDS (issued a whole stage ago) ...
     __syncthreads();                         // ... and so have the others'; and everyone is done with the other stage
-    t.step(s0, s1, rs, off, k + 1, k + 1 < k1, inside(k + 1), w, pa, qa, c0, c1);
+    t.step(s0, s1, a, p, p2, q, k + 1, k + 1 < k1, w, c0, c1);
     lds_t* x = s0; s0 = s1; s1 = x;
   }
+  __syncthreads();                           // the stages are free for the results
 
-  // a lane holds 4 consecutive columns of one output row: column 4 (lane / 16) + r, row lane % 16 of each 16 x 16 block
+  // a lane holds columns 4 (lane / 16) .. + 3 of row lane % 16 of each 16 x 16 block
+  lds_t* const out = (lds_t*)stage;
+  const int mw = wq * K::TQ + (lane & 15), nw = wp * (GATED ? K::TP / 2 : K::TP) + (lane >> 4) * 4;
+  const int rows = a.nq - m0, cols = a.np - n0;
+  constexpr int HI = GATED ? K::IP / 2 : 0, NI = GATED ? K::IP / 2 : K::IP;      // (accumulators of up: HI + i)
+  if (BP < 256 && a.splits > 1) {            // (the largest tile is taken only where there are many)
+    const int64_t width = GATED ? 2 * (int64_t)a.np : a.np;
+    float* base = a.slab + ((int64_t)blockIdx.y * a.nq + m0) * width + n0;
 #pragma unroll
-  for (int j = 0; j < K::IQ; ++j) {
-    const int m = m0 + wq * K::TQ + j * 16 + (lane & 15);
-    if (m >= a.nq) continue;
-    constexpr int HALF = EPI == EPI_GATED ? K::IP / 2 : K::IP;
+    for (int j = 0; j < K::IQ; ++j) {
+      const int m = mw + j * 16;
 #pragma unroll
-    for (int i = 0; i < HALF; ++i) {
-      const int n = n0 + wp * (EPI == EPI_GATED ? K::TP / 2 : K::TP) + i * 16 + (lane >> 4) * 4;
-      if (n >= a.np) continue;
-      if (a.splits > 1) {
-        const int64_t width = EPI == EPI_GATED ? 2 * (int64_t)a.np : a.np;
-        float* s = a.slab + ((int64_t)blockIdx.y * a.nq + m) * width + n;
-        const bool vec = (a.np & 3) == 0;
-        store4(s, t.acc[i][j], a.np - n, vec);
-        if (EPI == EPI_GATED) store4(s + a.np, t.acc[EPI == EPI_GATED ? i + K::IP / 2 : i][j], a.np - n, vec);
-      } else if (EPI == EPI_GATED) {
-        gated_out<O>(a, m, n, t.acc[i][j], t.acc[EPI == EPI_GATED ? i + K::IP / 2 : i][j]);
-      } else {
-        plain_out<O>(a, m, n, t.acc[i][j]);
+      for (int i = 0; i < K::IP; ++i) {
+        const int h = GATED && i >= HI ? 1 : 0, n = nw + (i - h * HI) * 16;
+        if (m < rows && n < cols) {
+          float* to = base + m * width + h * (int64_t)a.np + n;
+          if (n + 4 <= cols) *reinterpret_cast<Any16*>(to) = __builtin_bit_cast(Any16, t.acc[i][j]);
+          else put4(to, t.acc[i][j], cols - n);
+        }
+      }
+    }
+    return;
+  }
+  typedef O o4 __attribute__((ext_vector_type(4)));
+  if constexpr (!GATED) {
+    // in as many turns over the tile's rows as its results are larger than the two stages
+    constexpr int TURNS = (BQ * COLS * (int)sizeof(O) + 2 * K::STAGE - 1) / (2 * K::STAGE), R = BQ / TURNS;
+    typedef Out<O, R, COLS, NT> Z;
+    static_assert(Z::BYTES <= 2 * K::STAGE && (TURNS == 1 || TURNS == WQ), "a turn: the rows of one row of waves");
+    O* base = static_cast<O*>(a.out) + (int64_t)m0 * a.ldo + n0;
+#pragma unroll
+    for (int turn = 0; turn < TURNS; ++turn) {
+      if (TURNS == 1 || wq == turn) {
+#pragma unroll
+        for (int j = 0; j < K::IQ; ++j)
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+            const f32x4 v = t.acc[i][j] * a.alpha;
+            Z::put(out, mw + j * 16 - turn * R, nw + i * 16, o4{(O)v[0], (O)v[1], (O)v[2], (O)v[3]});
+          }
+      }
+      __syncthreads();
+      Z::store(out, base + (int64_t)turn * R * a.ldo, a.ldo, rows - turn * R, cols);
+      if (turn + 1 < TURNS) __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int n = n0 + nw + i * 16, last = a.np - 1;
+      const O* bias = static_cast<const O*>(a.bias);
+      f32x4 sg, su, bg, bu;
+      sg = su = f32x4{a.alpha, a.alpha, a.alpha, a.alpha};
+      bg = bu = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (a.sp) { sg *= four_of(a.sp, n, last); su *= four_of(a.sp + a.np, n, last); }
+      if (bias) { bg = four_of(bias, n, last); bu = four_of(bias + a.np, n, last); }
+#pragma unroll
+      for (int j = 0; j < K::IQ; ++j) {
+        const float q = a.sq ? a.sq[min(m0 + mw + j * 16, a.nq - 1)] : 1.f;
+        t.acc[i][j] = t.acc[i][j] * (sg * q) + bg;
+        t.acc[HI + i][j] = t.acc[HI + i][j] * (su * q) + bu;
+      }
+    }
+    typedef Out<O, BQ, COLS, NT> Z;
+    static_assert(Z::BYTES <= 2 * K::STAGE, "the results fit the stages");
+    auto put_out = [&](auto act) {
+#pragma unroll
+      for (int j = 0; j < K::IQ; ++j)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const f32x4 v = gate<decltype(act)::value>(t.acc[i][j], t.acc[HI + i][j]);
+          Z::put(out, mw + j * 16, nw + i * 16, o4{(O)v[0], (O)v[1], (O)v[2], (O)v[3]});
+        }
+    };
+    if (a.act == CAGC_ACT_SILU) put_out(std::integral_constant<int, CAGC_ACT_SILU>{});
+    else put_out(std::integral_constant<int, CAGC_ACT_GELU>{});
+    __syncthreads();
+    Z::store(out, static_cast<O*>(a.out) + (int64_t)m0 * a.ldo + n0, a.ldo, rows, cols);
+    if (!a.saved) return;
+    const int64_t plane = (int64_t)a.nq * a.np, first = (int64_t)m0 * a.np + n0;
+    if constexpr (sizeof(O) == 4) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < K::IQ; ++j)
+#pragma unroll
+          for (int i = 0; i < NI; ++i) Z::put(out, mw + j * 16, nw + i * 16, t.acc[h * HI + i][j]);
+        __syncthreads();
+        Z::store(out, static_cast<float*>(a.saved) + h * plane + first, a.np, rows, cols);
+      }
+    } else {
+      typedef Out<uint16_t, BQ, COLS, NT> S;
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+      uint16_t* saved = static_cast<uint16_t*>(a.saved) + first;
+#pragma unroll
+      for (int h = 0; h < 3; ++h) {            // two places in turn: one barrier a plane
+        lds_t* const at = 2 * S::BYTES <= 2 * K::STAGE ? out + (h & 1 ? 0 : S::BYTES) : out;
+        if (2 * S::BYTES > 2 * K::STAGE) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < K::IQ; ++j)
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+            const f32x4 g = t.acc[i][j], u = t.acc[HI + i][j];
+            const u32x2 v = h == 0 ? u32x2{upper2(g[0], g[1]), upper2(g[2], g[3])}
+                                   : (h == 1 ? u32x2{upper2(u[0], u[1]), upper2(u[2], u[3])} : u32x2{third2(g[0], u[0], g[1], u[1]), third2(g[2], u[2], g[3], u[3])});
+            S::put(at, mw + j * 16, nw + i * 16, __builtin_bit_cast(typename S::e4, v));
+          }
+        __syncthreads();
+        S::store(at, saved + h * plane, a.np, rows, cols);
       }
     }
   }
+}
+
+// the gated epilogue for the (up to) four outputs [m][n .. n+3], straight to memory
+template <class O> __device__ __forceinline__ void gated_out(const Product& a, int m, int n, f32x4 g, f32x4 u) {
+  const int left = a.np - n, last = a.np - 1;
+  const float q = a.alpha * (a.sq ? a.sq[m] : 1.f);
+  const O* bias = static_cast<const O*>(a.bias);
+  g *= a.sp ? four_of(a.sp, n, last) * q : f32x4{q, q, q, q};
+  u *= a.sp ? four_of(a.sp + a.np, n, last) * q : f32x4{q, q, q, q};
+  if (bias) { g += four_of(bias, n, last); u += four_of(bias + a.np, n, last); }
+  put4(static_cast<O*>(a.out) + (int64_t)m * a.ldo + n, a.act == CAGC_ACT_SILU ? gate<CAGC_ACT_SILU>(g, u) : gate<CAGC_ACT_GELU>(g, u), left);
+  if (!a.saved) return;
+  const int64_t plane = (int64_t)a.nq * a.np, i = (int64_t)m * a.np + n;
+  if (sizeof(O) == 4) {
+    put4(static_cast<float*>(a.saved) + i, g, left);
+    put4(static_cast<float*>(a.saved) + plane + i, u, left);
+    return;
+  }
+  uint16_t* s = static_cast<uint16_t*>(a.saved) + i;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (r < left) {
+      s[r] = (uint16_t)(bits(g[r]) >> 16);
+      s[plane + r] = (uint16_t)(bits(u[r]) >> 16);
+      s[2 * plane + r] = (uint16_t)((bits(g[r]) & 0xff00u) | ((bits(u[r]) >> 8) & 0xffu));
+    }
 }
 
 // the pieces of a K split, added in order, and the epilogue: four outputs a thread
@@ -234,13 +405,12 @@ template <class O, int EPI> __global__ __launch_bounds__(256) void k_join(Produc
     }
   }
   if (EPI == EPI_GATED) gated_out<O>(a, m, n, v[0], v[1]);
-  else plain_out<O>(a, m, n, v[0]);
+  else put4(static_cast<O*>(a.out) + (int64_t)m * a.ldo + n, v[0] * a.alpha, left);
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------------------------
 // Up to 16 MQ rows of x: bound by the weights' bytes, each read once, straight into registers.  A workgroup makes 16 output columns (16 gate
 // and 16 up rows); its waves share out K and are added through LDS.  Rows need no alignment: the loads are 16 bytes from any address.
-struct __attribute__((packed, aligned(1))) Any16 { uint32_t v[4]; };
 __device__ __forceinline__ i32x4 chunk_at(const char* row, int64_t at, int64_t kbytes) {
   if (at + 16 <= kbytes) return __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(row + at));
   union { uint8_t b[16]; i32x4 v; } u;
@@ -315,70 +485,83 @@ __global__ __launch_bounds__(256) void k_pad_rows(char* __restrict__ dst, const 
   const int64_t r = id / width16, c = (id % width16) * 16;
   *reinterpret_cast<i32x4*>(dst + (r * width16 * 16 + c)) = chunk_at(src + r * ld, c, kbytes);
 }
-// [rows, cols] -> [cols, ldd], zeros behind the last row's column up to ldd (elements; ldd >= rows)
-template <class E> __global__ __launch_bounds__(256) void k_transpose(E* __restrict__ dst, const E* __restrict__ src, int rows, int cols, int64_t lds_, int64_t ldd) {
-  __shared__ E t[64][65];
-  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int i = y; i < 64; i += 4) t[i][x] = (r0 + i < rows && c0 + x < cols) ? src[(int64_t)(r0 + i) * lds_ + c0 + x] : E(0);
-  __syncthreads();
-  for (int i = y; i < 64; i += 4)
-    if (c0 + i < cols && r0 + x < ldd) dst[(int64_t)(c0 + i) * ldd + r0 + x] = t[x][i];
-}
-
-// dz from the saved pre-activations and dy, in both layouts: z [rows, ldz] (zeros behind 2n) and zt [2n, ldzt] (zeros behind rows), and the
-// column sums of each band of 64 rows for db.  A workgroup makes 64 rows x 64 columns, gate and up.
-template <class T> __global__ __launch_bounds__(256) void k_dz(T* __restrict__ z, T* __restrict__ zt, float* __restrict__ dbpart, const T* __restrict__ dy, int64_t lddy,
-                                                              const void* __restrict__ saved, int rows, int n, int64_t ldz, int64_t ldzt, int act) {
-  __shared__ T t[2][64][65];
-  __shared__ float col[4][2][64];
-  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const int64_t plane = (int64_t)rows * n;
-  float sg = 0.f, su = 0.f;
-  for (int i = y; i < 64; i += 4) {
-    float dg = 0.f, du = 0.f;
-    const int64_t at = (int64_t)(r0 + i) * n + c0 + x;
-    if (r0 + i < rows && c0 + x < n) {
-      float g, u, a, da;
-      if (sizeof(T) == 4) {
-        g = static_cast<const float*>(saved)[at];
-        u = static_cast<const float*>(saved)[plane + at];
+// dz [rows, ldz] from the saved pre-activations and dy (zeros behind 2n), 8 or 4 columns a thread (16 bytes of dz), and the column sums of a band of rows
+// for db.  Bound by its bytes: dy, 3 planes of 16 bits (2 of fp32) and dz's two halves.
+constexpr int BAND = 64;      // rows of a workgroup
+template <class T> __global__ __launch_bounds__(256) void k_dz(T* __restrict__ z, float* __restrict__ dbpart, const T* __restrict__ dy, int64_t lddy, const void* __restrict__ saved,
+                                                              int rows, int n, int64_t ldz, int act) {
+  constexpr int V = 16 / (int)sizeof(T), GROUPS = 32;      // 32 threads side by side, 8 rows at a time
+  __shared__ float join[8][GROUPS][2 * V + 1];
+  const int x = threadIdx.x % GROUPS, y = threadIdx.x / GROUPS;
+  const int64_t c = ((int64_t)blockIdx.x * GROUPS + x) * V, plane = (int64_t)rows * n, left = n - c;
+  const int r0 = blockIdx.y * BAND, r1 = min(rows, r0 + BAND);
+  float sg[V], su[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sg[i] = su[i] = 0.f;
+  if (left > 0)
+    for (int r = r0 + y; r < r1; r += 8) {
+      const int64_t at = (int64_t)r * n + c;
+      float d[V], g[V], u[V];
+      load_v<V>(d, dy + r * lddy + c, left);
+      if constexpr (sizeof(T) == 4) {
+        load_v<V>(g, static_cast<const float*>(saved) + at, left);
+        load_v<V>(u, static_cast<const float*>(saved) + plane + at, left);
       } else {
         const uint16_t* s = static_cast<const uint16_t*>(saved) + at;
-        const uint32_t lo = s[2 * plane];
-        g = from24(s[0], lo >> 8);
-        u = from24(s[plane], lo & 0xffu);
+        uint16_t hg[V], hu[V], lo[V];
+        if (left >= V) {
+          const Any16 a = *reinterpret_cast<const Any16*>(s), b = *reinterpret_cast<const Any16*>(s + plane), l = *reinterpret_cast<const Any16*>(s + 2 * plane);
+          __builtin_memcpy(hg, &a, 16); __builtin_memcpy(hu, &b, 16); __builtin_memcpy(lo, &l, 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            hg[i] = i < left ? s[i] : 0; hu[i] = i < left ? s[plane + i] : 0; lo[i] = i < left ? s[2 * plane + i] : 0;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) { g[i] = from24(hg[i], lo[i] >> 8); u[i] = from24(hu[i], lo[i] & 0xffu); }
       }
-      const float d = (float)dy[(int64_t)(r0 + i) * lddy + c0 + x];
-      act_grad(act, g, a, da);
-      dg = d * u * da;
-      du = d * a;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float a, da;
+        act_grad(act, g[i], a, da);
+        const float dg = d[i] * u[i] * da, du = d[i] * a;
+        sg[i] += i < left ? dg : 0.f; su[i] += i < left ? du : 0.f;
+        g[i] = dg; u[i] = du;
+      }
+      if (z) {
+        T* p = z + r * ldz;
+        store_v<V>(p + c, g, left);
+        store_v<V>(p + n + c, u, left);
+        if (left <= V) for (int64_t i = 2 * (int64_t)n; i < ldz; ++i) p[i] = (T)0.f;
+      }
     }
-    sg += dg; su += du;
-    t[0][i][x] = (T)dg; t[1][i][x] = (T)du;
-    if (z && r0 + i < rows) {
-      T* p = z + (int64_t)(r0 + i) * ldz;
-      if (c0 + x < n) { p[c0 + x] = (T)dg; p[n + c0 + x] = (T)du; }
-      if (c0 + x < ldz - 2 * n) p[2 * n + c0 + x] = (T)0.f;
-    }
-  }
-  col[y][0][x] = sg; col[y][1][x] = su;
+  if (!dbpart) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) { join[y][x][i] = sg[i]; join[y][x][V + i] = su[i]; }
   __syncthreads();
-  if (dbpart && threadIdx.x < 128) {
-    const int h = threadIdx.x >> 6;
-    if (c0 + x < n) dbpart[(int64_t)blockIdx.y * 2 * n + h * n + c0 + x] = (col[0][h][x] + col[1][h][x]) + (col[2][h][x] + col[3][h][x]);
+  for (int id = threadIdx.x; id < GROUPS * 2 * V; id += 256) {
+    const int g = id / (2 * V), i = id % (2 * V);
+    const int64_t col = ((int64_t)blockIdx.x * GROUPS + g) * V + i % V;
+    if (col >= n) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += join[k][g][i];
+    dbpart[(int64_t)blockIdx.y * 2 * n + (i / V) * n + col] = s;
   }
-  if (!zt) return;
-  for (int i = y; i < 64; i += 4)
-    if (c0 + i < n && r0 + x < ldzt) {
-      zt[(int64_t)(c0 + i) * ldzt + r0 + x] = t[0][x][i];
-      zt[(int64_t)(n + c0 + i) * ldzt + r0 + x] = t[1][x][i];
-    }
 }
-template <class T> __global__ __launch_bounds__(256) void k_db(T* __restrict__ db, const float* __restrict__ part, int bands, int cols) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+// db[c] = sum of the bands' shares, in a fixed order
+template <class T> __global__ __launch_bounds__(1024) void k_db(T* __restrict__ db, const float* __restrict__ part, int bands, int cols) {
+  __shared__ float sh[16][64];
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6, c = blockIdx.x * 64 + x;
   float s = 0.f;
-  for (int b = 0; b < bands; ++b) s += part[(int64_t)b * cols + c];
+  if (c < cols)
+#pragma unroll 4
+    for (int b = y; b < bands; b += 16) s += part[(int64_t)b * cols + c];
+  sh[y][x] = s;
+  __syncthreads();
+  if (y || c >= cols) return;
+  for (int i = 1; i < 16; ++i) s += sh[i][x];
   db[c] = (T)s;
 }
 
@@ -404,17 +587,17 @@ Plan plan_of(bool gated, int64_t rows, int64_t cols, int ksteps) {
   return p;
 }
 
-template <class T, class O, int EPI> int launch_product(Product& a, const Plan& p, hipStream_t st, const char* what) {
+template <class T, class O, int EPI, bool DP = false, bool DQ = false> int launch_product(Product& a, const Plan& p, hipStream_t st, const char* what) {
   const int cols = EPI == EPI_GATED ? p.bp / 2 : p.bp;
   a.tiles_p = cdiv(a.np, cols);
   a.tiles_q = cdiv(a.nq, p.bq);
   const int per = cdiv(a.ksteps, p.splits);
   a.splits = cdiv(a.ksteps, per);          // no empty piece
   const dim3 grid((unsigned)(a.tiles_p * a.tiles_q), (unsigned)a.splits);
-  if (p.bp == 256) hipLaunchKernelGGL((k_product<T, O, 256, 256, 4, 2, EPI>), grid, dim3(512), 0, st, a);
-  else if (p.bq == 128) hipLaunchKernelGGL((k_product<T, O, 128, 128, 2, 2, EPI>), grid, dim3(256), 0, st, a);
-  else if (p.bq == 64) hipLaunchKernelGGL((k_product<T, O, 128, 64, 4, 1, EPI>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_product<T, O, 128, 32, 4, 1, EPI>), grid, dim3(256), 0, st, a);
+  if (p.bp == 256) hipLaunchKernelGGL((k_product<T, O, 256, 256, 4, 2, EPI, DP, DQ>), grid, dim3(512), 0, st, a);
+  else if (p.bq == 128) hipLaunchKernelGGL((k_product<T, O, 128, 128, 2, 2, EPI, DP, DQ>), grid, dim3(256), 0, st, a);
+  else if (p.bq == 64) hipLaunchKernelGGL((k_product<T, O, 128, 64, 4, 1, EPI, DP, DQ>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_product<T, O, 128, 32, 4, 1, EPI, DP, DQ>), grid, dim3(256), 0, st, a);
   int rc = check_launch(what);
   if (rc != CAGC_OK || a.splits == 1) return rc;
   const int64_t quads = (int64_t)((a.np + 3) / 4) * a.nq;
@@ -467,44 +650,44 @@ bool sizes_ok(int64_t rows, int64_t n, int64_t k, int dtype) {
   return rows >= 0 && n > 0 && k > 0 && rows < (1ll << 31) - 512 && n < (1 << 29) && k * esize(dtype) <= MOST_LD;
 }
 
-struct BwdLayout { int64_t z, zt, wt, xt, dbpart, slab, total; int64_t ldz, ldm; Plan dx, dw; };
-BwdLayout bwd_layout(int64_t rows, int64_t n, int64_t k, int dtype, bool need_dx, bool need_dw, bool need_db) {
+struct BwdLayout { int64_t z, wpad, xpad, dbpart, slab, total; int64_t ldz, kpad; Plan dx, dw; };
+BwdLayout bwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, int dtype, bool need_dx, bool need_dw, bool need_db) {
   BwdLayout l = {};
-  const int e = esize(dtype), v = 16 / e;
+  const int e = esize(dtype), v = 16 / e, rk = 128 / e;
   l.ldz = (2 * n + v - 1) / v * v;
-  l.ldm = (rows + v - 1) / v * v;
-  int64_t at = 0;
-  if (need_dx) { l.z = at; at += up256(rows * l.ldz * e); l.wt = at; at += up256(k * l.ldz * e); l.dx = plan_of(false, rows, k, (int)((l.ldz * e + 127) / 128)); }
-  if (need_dw) { l.zt = at; at += up256(2 * n * l.ldm * e); l.xt = at; at += up256(k * l.ldm * e); l.dw = plan_of(false, 2 * n, k, (int)((l.ldm * e + 127) / 128)); }
-  if (need_db) { l.dbpart = at; at += up256(4 * ((rows + 63) / 64) * 2 * n); }
+  l.kpad = up16(k * e);
+  int64_t at = 0, s = 0;
+  if (need_dx || need_dw) at += up256(rows * l.ldz * e);
+  if (need_dx) {
+    l.dx = plan_of(false, rows, k, (int)((2 * n + rk - 1) / rk));
+    if (!w_ok) { l.wpad = at; at += up256(2 * n * l.kpad); }
+    if (l.dx.splits > 1) s = 4 * (int64_t)l.dx.splits * rows * k;
+  }
+  if (need_dw) {
+    l.dw = plan_of(false, 2 * n, k, (int)((rows + rk - 1) / rk));
+    if (!x_ok) { l.xpad = at; at += up256(rows * l.kpad); }
+    const int64_t t = l.dw.splits > 1 ? 4 * (int64_t)l.dw.splits * 2 * n * k : 0;
+    if (t > s) s = t;
+  }
+  if (need_db) { l.dbpart = at; at += up256(4 * ((rows + BAND - 1) / BAND) * 2 * n); }
   l.slab = at;
-  int64_t s = 0;
-  if (need_dx && l.dx.splits > 1) s = 4 * (int64_t)l.dx.splits * rows * k;
-  if (need_dw && l.dw.splits > 1) { const int64_t t = 4 * (int64_t)l.dw.splits * 2 * n * k; if (t > s) s = t; }
   l.total = at + up256(s);
   return l;
 }
 
-template <class E> int transpose(void* dst, const void* src, int64_t rows, int64_t cols, int64_t ld, int64_t ldd, hipStream_t st, const char* what) {
-  const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)((ldd + 63) / 64));
-  hipLaunchKernelGGL((k_transpose<E>), grid, dim3(256), 0, st, (E*)dst, (const E*)src, (int)rows, (int)cols, ld, ldd);
-  return check_launch(what);
-}
-
 template <class T> int backward(void* dx, void* dw, void* db, char* ws, const void* dy, const void* saved, const void* x, const void* w, int64_t rows, int64_t n,
                                 int64_t k, int64_t ldx, int64_t ldw, int64_t lddy, int dtype, int act, float scale, hipStream_t st, const char* what) {
-  typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type E;
-  const int e = sizeof(T);
-  const BwdLayout l = bwd_layout(rows, n, k, dtype, dx != nullptr, dw != nullptr, db != nullptr);
-  T* z = dx ? (T*)(ws + l.z) : nullptr;
-  T* zt = dw ? (T*)(ws + l.zt) : nullptr;
+  const int e = sizeof(T), v = 16 / e, rk = 128 / e;
+  const bool x_ok = !dw || aligned(x, ldx * e, k * e), w_ok = !dx || aligned(w, ldw * e, k * e);
+  const BwdLayout l = bwd_layout(rows, n, k, x_ok, w_ok, dtype, dx != nullptr, dw != nullptr, db != nullptr);
+  T* z = dx || dw ? (T*)(ws + l.z) : nullptr;
   float* part = db ? (float*)(ws + l.dbpart) : nullptr;
-  const int bands = cdiv(dw ? l.ldm : rows, 64);
-  hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)((n + 63) / 64), (unsigned)bands), dim3(256), 0, st, z, zt, part, (const T*)dy, lddy, saved, (int)rows, (int)n, l.ldz, l.ldm, act);
+  const int bands = cdiv(rows, BAND);
+  hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)((n + 32 * v - 1) / (32 * v)), (unsigned)bands), dim3(256), 0, st, z, part, (const T*)dy, lddy, saved, (int)rows, (int)n, l.ldz, act);
   int rc = check_launch(what);
   if (rc != CAGC_OK) return rc;
   if (db) {
-    hipLaunchKernelGGL((k_db<T>), dim3((unsigned)((2 * n + 255) / 256)), dim3(256), 0, st, (T*)db, part, cdiv(rows, 64), (int)(2 * n));
+    hipLaunchKernelGGL((k_db<T>), dim3((unsigned)((2 * n + 63) / 64)), dim3(1024), 0, st, (T*)db, part, bands, (int)(2 * n));
     if ((rc = check_launch(what)) != CAGC_OK) return rc;
   }
   Product a = {};
@@ -512,23 +695,22 @@ template <class T> int backward(void* dx, void* dw, void* db, char* ws, const vo
   a.slab = (float*)(ws + l.slab);
   a.ldo = k;
   a.np = (int)k;
-  if (dx) {
-    if ((rc = transpose<E>(ws + l.wt, w, 2 * n, k, ldw, l.ldz, st, what)) != CAGC_OK) return rc;
-    a.p = ws + l.wt; a.p2 = a.p; a.ldp = l.ldz * e;
-    a.q = (const char*)z; a.ldq = l.ldz * e;
+  a.q = (const char*)z; a.ldq = l.ldz * e;
+  if (dx) {                                  // dz [rows, 2n] along its rows, W [2n, k] down its columns
+    a.p = (const char*)w; a.ldp = ldw * e;
+    if (!w_ok) { if ((rc = pad_rows(ws + l.wpad, w, 2 * n, k * e, ldw * e, st, what)) != CAGC_OK) return rc; a.p = ws + l.wpad; a.ldp = l.kpad; }
     a.nq = (int)rows;
-    a.kbytes = (int)(l.ldz * e); a.ksteps = cdiv(a.kbytes, 128);
+    a.kbytes = (int)(l.ldz * e); a.krows = (int)(2 * n); a.ksteps = cdiv(2 * n, rk);
     a.out = dx;
-    if ((rc = launch_product<T, T, EPI_PLAIN>(a, l.dx, st, what)) != CAGC_OK) return rc;
+    if ((rc = launch_product<T, T, EPI_PLAIN, true, false>(a, l.dx, st, what)) != CAGC_OK) return rc;
   }
-  if (dw) {
-    if ((rc = transpose<E>(ws + l.xt, x, rows, k, ldx, l.ldm, st, what)) != CAGC_OK) return rc;
-    a.p = ws + l.xt; a.p2 = a.p; a.ldp = l.ldm * e;
-    a.q = (const char*)zt; a.ldq = l.ldm * e;
+  if (dw) {                                  // dz and x [rows, k] down their columns
+    a.p = (const char*)x; a.ldp = ldx * e;
+    if (!x_ok) { if ((rc = pad_rows(ws + l.xpad, x, rows, k * e, ldx * e, st, what)) != CAGC_OK) return rc; a.p = ws + l.xpad; a.ldp = l.kpad; }
     a.nq = (int)(2 * n);
-    a.kbytes = (int)(l.ldm * e); a.ksteps = cdiv(a.kbytes, 128);
+    a.kbytes = 0; a.krows = (int)rows; a.ksteps = cdiv(rows, rk);
     a.out = dw;
-    if ((rc = launch_product<T, T, EPI_PLAIN>(a, l.dw, st, what)) != CAGC_OK) return rc;
+    if ((rc = launch_product<T, T, EPI_PLAIN, true, true>(a, l.dw, st, what)) != CAGC_OK) return rc;
   }
   return CAGC_OK;
 }
@@ -587,9 +769,11 @@ extern "C" int cagc_gated_linear_fwd(void* out, void* saved, void* ws, const voi
   return forward<e4m3, __bf16>(a, l, st, what);
 }
 
-extern "C" int64_t cagc_gated_linear_bwd_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int need_dx, int need_dw, int need_db) {
+extern "C" int64_t cagc_gated_linear_bwd_workspace(const void* x, const void* w, int64_t rows, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int dtype, int need_dx, int need_dw,
+                                                   int need_db) {
   if (!sizes_ok(rows, n, k, dtype)) return 0;
-  return bwd_layout(rows, n, k, dtype, need_dx, need_dw, need_db).total;
+  const int64_t e = esize(dtype);
+  return bwd_layout(rows, n, k, aligned(x, ldx * e, k * e), aligned(w, ldw * e, k * e), dtype, need_dx, need_dw, need_db).total;
 }
 
 extern "C" int cagc_gated_linear_bwd(void* dx, void* dw, void* db, void* ws, const void* dy, const void* saved, const void* x, const void* w, int64_t rows, int64_t n,

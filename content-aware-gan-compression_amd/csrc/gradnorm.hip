@@ -5,7 +5,7 @@
 // GROUP tensors a launch: no table to upload, so a captured launch holds its own), a workgroup takes one piece of one tensor.
 // Sums run in 64 bits (squares of fp32 and bf16 values leave the range of fp32, and a billion of them its precision), in a fixed order: the
 // pieces' sums go to the workspace, one workgroup adds them.
-#include "common.h"
+#include "rows.h"
 #include <stdlib.h>
 
 namespace cagc {
@@ -23,8 +23,6 @@ struct Group {
   const float* coef;
 };
 static_assert(sizeof(Group) <= 4000, "kernel arguments");
-
-struct __attribute__((packed, aligned(1))) Any16 { uint32_t v[4]; };
 
 // magnitudes as bit patterns: a NaN is above infinity and so is kept
 __device__ __forceinline__ double larger(double a, double b) {

@@ -4,49 +4,14 @@
 //   backward, with t = dy w and n = h rstd:  dx = dresidual = rstd (t - n mean(t n)) + dh,   dw = sum over rows of dy n
 //
 // Bound by HBM: a row is read once and kept in registers between its sums and its output (TPR threads a row, NV chunks of 16 bytes each),
-// so a forward moves x, residual, h and y once.  Sums are fp32.  Rows may start at any address: the 16-byte loads need no alignment, only the
-// chunk that crosses a row's end goes element by element.
-#include "common.h"
+// so a forward moves x, residual, h and y once.  Sums are fp32.  Rows may start at any address.
+#include "rows.h"
 
 namespace cagc {
 namespace {
 
-struct __attribute__((packed, aligned(1))) Any16 { uint32_t v[4]; };
-
 template <class T> struct Row { static constexpr int V = 16 / (int)sizeof(T); };
 
-// V elements from p (any alignment) as floats; those from `left` on are zero and not read
-template <int V, class T> __device__ __forceinline__ void load_v(float (&f)[V], const T* p, int64_t left) {
-  T e[V];
-  if (left >= V) {
-    constexpr int N = V * (int)sizeof(T) / 16;
-    static_assert(N >= 1, "whole 16-byte pieces");
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const Any16 a = reinterpret_cast<const Any16*>(p)[i];
-      __builtin_memcpy(reinterpret_cast<char*>(e) + 16 * i, &a, 16);
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = (float)e[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = i < left ? (float)p[i] : 0.f;
-  }
-}
-template <int V, class T> __device__ __forceinline__ void store_v(T* p, const float (&f)[V], int64_t left) {
-  if (left >= V) {
-    T e[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = (T)f[i];
-    Any16 a;
-    static_assert(V * sizeof(T) == 16, "one 16-byte piece");
-    __builtin_memcpy(&a, e, 16);
-    *reinterpret_cast<Any16*>(p) = a;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) if (i < left) p[i] = (T)f[i];
-  }
-}
 // V e4m3 bytes
 template <int V> __device__ __forceinline__ void store_q(uint8_t* p, const float (&f)[V], float inv, int64_t left) {
   uint32_t d[V / 4];

@@ -565,7 +565,8 @@ int cagc_gated_linear_fwd(void* out, void* saved /*[nullable]*/, void* ws, const
                           int64_t ldx, int64_t ldw, int dtype, int out_dtype, int act, float scale, cagc_stream_t stream);
 /* dx [rows, k], dw [2n, k], db [2n] (each nullable: not wanted), contiguous, in dtype; dy [rows, n] with rows lddy apart.  rows > 0.  Every sum runs in
  * a fixed order: two calls give the same bits. */
-int64_t cagc_gated_linear_bwd_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int need_dx, int need_dw, int need_db);
+int64_t cagc_gated_linear_bwd_workspace(const void* x, const void* w, int64_t rows, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int dtype, int need_dx,
+                                        int need_dw, int need_db);
 int cagc_gated_linear_bwd(void* dx, void* dw, void* db, void* ws, const void* dy, const void* saved, const void* x, const void* w, int64_t rows,
                           int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t lddy, int dtype, int act, float scale, cagc_stream_t stream);
 

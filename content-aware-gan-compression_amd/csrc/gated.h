@@ -18,31 +18,26 @@ template <> struct Type<_Float16> { static constexpr int size = 2; };
 template <> struct Type<__bf16> { static constexpr int size = 2; };
 template <> struct Type<e4m3> { static constexpr int size = 1; };
 
-// One matrix-core step over the 128 bytes of K that a stage holds of a row.  A lane brings the 16-byte chunks number lane/16 and
-// 4 + lane/16 of its row (lane % 16) of either operand; which k a chunk's elements are does not matter as long as both operands
-// agree, so one addressing serves 2 products of 16x16x32 (16-bit), 8 of 16x16x4 (fp32) and 1 of 16x16x128 (e4m3).
-template <class T> __device__ __forceinline__ f32x4 mma(const i32x4 (&a)[2], const i32x4 (&b)[2], f32x4 c);
-template <> __device__ __forceinline__ f32x4 mma<__bf16>(const i32x4 (&a)[2], const i32x4 (&b)[2], f32x4 c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[0]), __builtin_bit_cast(bf16x8, b[0]), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[1]), __builtin_bit_cast(bf16x8, b[1]), c, 0, 0, 0);
+// One matrix-core step over the 64 bytes of K (e4m3: 128) that a piece of a stage holds of a row.  A lane brings the 16-byte chunk number lane / 16 (e4m3: and 4 + lane / 16) of
+// its row (lane % 16) of either operand; which k a chunk's elements are does not matter as long as both operands agree, so one addressing serves one product of 16x16x32 (16-bit), 4 of
+// 16x16x4 (fp32) and one of 16x16x128 (e4m3, no block scales).
+template <class T> struct Piece { typedef i32x4 type; static constexpr int count = 2; };      // a lane's part of a piece; pieces in 128 bytes
+template <> struct Piece<e4m3> { typedef i32x8 type; static constexpr int count = 1; };
+template <class T> __device__ __forceinline__ f32x4 mma(typename Piece<T>::type a, typename Piece<T>::type b, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mma<__bf16>(i32x4 a, i32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ f32x4 mma<_Float16>(const i32x4 (&a)[2], const i32x4 (&b)[2], f32x4 c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[0]), __builtin_bit_cast(f16x8, b[0]), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[1]), __builtin_bit_cast(f16x8, b[1]), c, 0, 0, 0);
+template <> __device__ __forceinline__ f32x4 mma<_Float16>(i32x4 a, i32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ f32x4 mma<float>(const i32x4 (&a)[2], const i32x4 (&b)[2], f32x4 c) {
+template <> __device__ __forceinline__ f32x4 mma<float>(i32x4 a, i32x4 b, f32x4 c) {
+  const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x4 x = __builtin_bit_cast(f32x4, a[h]), y = __builtin_bit_cast(f32x4, b[h]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-  }
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
   return c;
 }
-template <> __device__ __forceinline__ f32x4 mma<e4m3>(const i32x4 (&a)[2], const i32x4 (&b)[2], f32x4 c) {
-  const i32x8 x = __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7), y = __builtin_shufflevector(b[0], b[1], 0, 1, 2, 3, 4, 5, 6, 7);
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);      // both e4m3, no block scales
-}
+template <> __device__ __forceinline__ f32x4 mma<e4m3>(i32x8 a, i32x8 b, f32x4 c) { return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0); }
+__device__ __forceinline__ i32x8 join(i32x4 a, i32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 // act(g) and act'(g).  SiLU: g s with s = 1 / (1 + e^-g), derivative s (1 + g (1 - s)); GELU: g Phi(g), derivative Phi(g) + g phi(g).
 // Phi by Abramowitz and Stegun's formula 7.1.26 (erf to 1.5e-7, so Phi to 0.8e-7, little over an fp32 rounding of 1): without branches, and its exponential is phi's

@@ -21,7 +21,6 @@ struct Product {
   int np, nq;            // columns and rows of the output
   int kbytes;            // K in bytes (a multiple of 16) where a row holds K ...
   int krows;             // ... and in rows where a column does
-  int ksteps;            // K in stages
   int splits;            // K is cut into this many pieces, each with a slab of its own
   int tiles_p, tiles_q;
   float* slab;           // [splits][nq][np or 2 np] fp32
@@ -40,19 +39,19 @@ template <class V> __device__ __forceinline__ V lds_read(const lds_t* p) { retur
 
 // ---- tiled product --------------------------------------------------------------------------------------------------------------
 // out[m][n] = sum_k q[m][k] p[n][k].  A workgroup of WP x WQ waves makes a tile of BQ rows (m) and BP rows of p (n; gated: BP/2 columns,
-// gate and up); K goes by in stages of 128 bytes a row, two stages in LDS: while one is multiplied, the other is filled by loads that
+// gate and up); K goes by in stages of SB bytes a row, NS stages in LDS: while one is multiplied, the next ones are filled by loads that
 // go straight to LDS, in lane order, 16 bytes a lane.
 //
 // An operand lies in memory with K along its rows (x, W in the forward), or with K down its columns (W for dx; dz and x for dW).  In LDS a stage keeps that
-// order: B rows of 128 bytes, or 128 / size rows of B elements.  Along rows, a wave reads 16 bytes of 16 rows at a time; down columns, the
+// order: B rows of SB bytes, or SB / size rows of B elements.  Along rows, a wave reads 16 bytes of 16 rows at a time; down columns, the
 // transposing read hands each lane 4 elements of a column (16-bit types), or it reads single elements (fp32).  Either way a lane ends up with the k that the other operand's lane
-// has: chunk number lane / 16 (and 4 + lane / 16) of the stage's eight.  So that those reads fall into different banks, chunk c of LDS row r is kept at c ^ turn(r).
+// has: chunk number lane / 16 (and 4 + lane / 16) of the stage's four (eight).  So that those reads fall into different banks, chunk c of LDS row r is kept at c ^ turn(r).
 // Nothing outside the operands is read: rows beyond the last repeat it (their outputs are not stored), chunks beyond a row and rows beyond K come back as zero.
-template <class T, int B, bool DOWN> struct Side {
-  static constexpr int ES = Type<T>::size, RK = 128 / ES;          // elements of K in a stage
-  static constexpr int ROW = DOWN ? B * ES : 128, CH = ROW / 16;   // bytes and chunks of an LDS row
+template <class T, int B, bool DOWN, int SB> struct Side {
+  static constexpr int ES = Type<T>::size, RK = SB / ES;           // elements of K in a stage
+  static constexpr int ROW = DOWN ? B * ES : SB, CH = ROW / 16;    // bytes and chunks of an LDS row
   static __device__ __forceinline__ int turn(int row) {
-    if (!DOWN) return row & 7;
+    if (!DOWN) return SB == 64 ? (row >> 2) & 3 : row & 7;
     if (ES == 2) return (((row & 3) | ((row >> 3) & 1) << 2) << 1) & (CH - 1);
     return (((row >> 2) & 3) << 2) & (CH - 1);
   }
@@ -70,7 +69,7 @@ template <class T, int B, bool DOWN> struct Side {
   // LDS address of this lane's part of the 16 columns / rows `t` (in sixteens)
   static __device__ __forceinline__ int place(int t, int lane) {
     const int g = lane >> 4, l = lane & 15;
-    if (!DOWN) return (t * 16 + l) * 128;
+    if (!DOWN) return (t * 16 + l) * SB;
     if (ES == 2) { const int row = 8 * g + (l >> 2); return row * ROW + (((2 * t) ^ turn(row)) + ((l & 3) >> 1)) * 16 + (l & 1) * 8; }
     const int row = 4 * g;
     return row * ROW + (((4 * t) ^ turn(row)) + (l >> 2)) * 16 + (l & 3) * 4;
@@ -93,46 +92,96 @@ template <class T, int B, bool DOWN> struct Side {
   }
 };
 
+// Stages.  Two of 128 bytes a row; with K down the columns of 16-bit operands, where a row of LDS is 512 contiguous bytes of memory whatever SB is, the largest tile takes five of 64, so that a load has
+// three stages' products to arrive in (dW of 8192 x 2048 -> 8192 bf16: 411 -> 396 us, with zeros for operands, which leave the clock alone, 376 -> 312).  Elsewhere five are slower: along rows a load
+// would fetch half lines (the forward of that: 432 -> 457 us), two smaller workgroups on a CU cover each other's waits (1024 x 2048 ...: 26 -> 31 us), and fp32's products take 16 times as long.
+template <class T, int BQ, bool DP> struct Stages {
+  static constexpr bool FIVE = DP && BQ == 256 && Type<T>::size == 2;
+  static constexpr int SB = FIVE ? 64 : 128, NS = FIVE ? 5 : 2;
+};
+
 template <class T, class O, int BP, int BQ, int WP, int WQ, int EPI, bool DP, bool DQ> struct Tile {      // (O: a class of its own for each kernel)
-  typedef Side<T, BP, DP> P;
-  typedef Side<T, BQ, DQ> Q;
+  static constexpr int SB = Stages<T, BQ, DP>::SB, NS = Stages<T, BQ, DP>::NS;
+  typedef Side<T, BP, DP, SB> P;
+  typedef Side<T, BQ, DQ, SB> Q;
   static constexpr int NW = WP * WQ, TP = BP / WP, TQ = BQ / WQ, IP = TP / 16, IQ = TQ / 16;
-  static constexpr int LP = BP / 8 / NW, LQ = BQ / 8 / NW;         // loads of 1 KB of a wave and stage
-  static constexpr int STAGE = (BP + BQ) * 128;
-  static_assert(BP % (16 * NW) == 0 && BQ % (8 * NW) == 0, "a wave's loads lie in one operand, and in one half of p");
+  static constexpr int LP = BP * SB / 1024 / NW, LQ = BQ * SB / 1024 / NW;         // loads of 1 KB of a wave and stage
+  static constexpr int STAGE = (BP + BQ) * SB, LDS = NS * STAGE;
+  static_assert(BP / 2 * SB % (1024 * NW) == 0 && BQ * SB % (1024 * NW) == 0, "a wave's loads lie in one operand, and in one half of p");
   f32x4 acc[IP][IQ];
   int pa[IP], qa[IQ];              // LDS places of this lane's operands
   int po[LP], qo[LQ];              // sources of this lane's loads
   int pk, qk;                      // Side::first of them
+  int ends_p, ends_q;              // where K ends, in rows of K (down columns) or bytes (along rows)
 
-  __device__ __forceinline__ void fill(lds_t* __restrict__ dst, const Product& a, const char* p, const char* p2, const char* q, int step, int w) {
-    const int pl = DP ? a.krows - step * P::RK : a.kbytes - step * 128, ql = DQ ? a.krows - step * Q::RK : a.kbytes - step * 128;      // what is left of K
-#pragma unroll
-    for (int c = 0; c < LP; ++c) {
-      const int at = c * NW * 1024;
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(!DP && at >= BP * 64 ? p2 : p), 0, 0x7ffffff0, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + at + w * 1024), 16,
-                                               pk + c * P::template further<NW>() < pl ? po[c] : (int)0x80000000, 0, 0, 0);
-    }
-#pragma unroll
-    for (int c = 0; c < LQ; ++c) {
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)q, 0, 0x7ffffff0, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + BP * 128 + c * NW * 1024 + w * 1024), 16,
-                                               qk + c * Q::template further<NW>() < ql ? qo[c] : (int)0x80000000, 0, 0, 0);
-    }
+  // load number c of this wave and stage `step`: zeros where K (of this split) has ended
+  __device__ __forceinline__ void load(lds_t* __restrict__ dst, int c, const char* p, const char* p2, const char* q, int step, int w) {
+    const bool is_p = c < LP;
+    const int at = is_p ? c * NW * 1024 : BP * SB + (c - LP) * NW * 1024;
+    const char* from = is_p ? (!DP && at >= BP / 2 * SB ? p2 : p) : q;
+    const bool ok = is_p ? pk + c * P::template further<NW>() < ends_p - step * (DP ? P::RK : SB) : qk + (c - LP) * Q::template further<NW>() < ends_q - step * (DQ ? Q::RK : SB);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, 0x7ffffff0, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(dst + at + w * 1024), 16, ok ? (is_p ? po[c < LP ? c : 0] : qo[c < LP ? 0 : c - LP]) : (int)0x80000000, 0, 0, 0);
   }
-  // (one function with both stages as restricted pointers: the compiler then knows that the loads into `nxt` do not touch what is read from `cur`, and does not wait for them)
-  __device__ __forceinline__ void step(lds_t* __restrict__ cur, lds_t* __restrict__ nxt, const Product& a, const char* p, const char* p2, const char* q, int next, bool more, int w,
-                                       int c0, int c1) {
-    if (more) fill(nxt, a, p, p2, q, next, w);
-    i32x4 pf[IP][2];
+  // A stage goes by in H pieces of K; of a piece, p's IP parts are held in registers while q's IQ parts pass.
+  typedef typename Piece<T>::type part;
+  static constexpr int H = SB / 128 * (Piece<T>::count - 1) + 1, N = H * IQ, L = LP + LQ;
+  static constexpr int LATE = IQ >= 4 ? (Type<T>::size > 1 ? 4 : 2) : IQ;      // parts of q read ahead, and multiplied behind the barrier
+  template <class S> static __device__ __forceinline__ part read(const lds_t* side, int at, int h, int c0, int c1) {
+    if constexpr (Piece<T>::count == 2) return S::read(side, at, h, h ? c1 : c0);
+    else return join(S::read(side, at, 0, c0), S::read(side, at, 1, c1));
+  }
+  __device__ __forceinline__ part read_q(const lds_t* stage, int k, int c0, int c1) { return read<Q>(stage + BP * SB, qa[k % IQ], k / IQ, c0, c1); }
+  // The first stages' loads, and the first reads (of stage 0, which `s0` is).
+  __device__ __forceinline__ void begin(lds_t* __restrict__ s0, lds_t* __restrict__ s1, part (&first)[IP], part (&ahead)[LATE], const char* p, const char* p2, const char* q, int64_t dp, int64_t dq,
+                                        int k0, int w, int c0, int c1) {
 #pragma unroll
-    for (int i = 0; i < IP; ++i) { pf[i][0] = P::read(cur, pa[i], 0, c0); pf[i][1] = P::read(cur, pa[i], 1, c1); }
+    for (int c = 0; c < L; ++c) load(s0, c, p, p2, q, k0, w);
 #pragma unroll
-    for (int j = 0; j < IQ; ++j) {
-      const i32x4 qf[2] = {Q::read(cur + BP * 128, qa[j], 0, c0), Q::read(cur + BP * 128, qa[j], 1, c1)};
+    for (int n = 1; n < NS; ++n)
 #pragma unroll
-      for (int i = 0; i < IP; ++i) acc[i][j] = mma<T>(pf[i], qf, acc[i][j]);
+      for (int c = 0; c < L; ++c) load(s1 + (n - 1) * STAGE, c, p + n * dp, p2 + n * dp, q + n * dq, k0 + n, w);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * L) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < IP; ++i) first[i] = read<P>(s0, pa[i], 0, c0, c1);
+#pragma unroll
+    for (int k = 0; k < LATE; ++k) ahead[k] = read_q(s0, k, c0, c1);
+  }
+  // One stage, in `cur`; the first piece of p is in `first`, the first parts of q in `ahead`.  q is read LATE parts ahead, each read and load between the products of one part and the next (the order is
+  // pinned).  When the barrier comes, all of the stage has been read, and behind it the next one is in `nxt` for everyone and `cur` is free: the loads of the stage NS further on and the next stage's first
+  // reads run under the last LATE parts' products.
+  // (One function with both stages as restricted pointers: the compiler then knows that the loads do not touch what is read, and does not wait for them.)
+  __device__ __forceinline__ void step(lds_t* __restrict__ cur, lds_t* __restrict__ nxt, part (&first)[IP], part (&then)[IP], part (&ahead)[LATE], const char* p, const char* p2, const char* q, int far,
+                                       int w, int c0, int c1) {
+    part last[IP], qf[N];
+#pragma unroll
+    for (int k = 0; k < LATE; ++k) qf[k] = ahead[k];
+#pragma unroll
+    for (int k = 0; k < N - LATE; ++k) {
+      qf[k + LATE] = read_q(cur, k + LATE, c0, c1);
+      if (H == 2 && k < IP) last[k] = read<P>(cur, pa[k < IP ? k : 0], 1, c0, c1);
+      if (H == 2 && k == N - LATE - 1) {
+#pragma unroll
+        for (int i = k + 1; i < IP; ++i) last[i] = read<P>(cur, pa[i], 1, c0, c1);
+      }
+#pragma unroll
+      for (int i = 0; i < IP; ++i) acc[i][k % IQ] = mma<T>(H == 2 && k >= IQ ? last[i] : first[i], qf[k], acc[i][k % IQ]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // this wave's loads of the next stage have reached LDS (those of the NS - 2 behind it may be on their way), its reads are done; and so are the others'
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * L) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int l = 0; l < LATE; ++l) {
+      ahead[l] = read_q(nxt, l, c0, c1);
+#pragma unroll
+      for (int i = 0; i < IP; ++i) if (i * LATE / IP == l) then[i] = read<P>(nxt, pa[i], 0, c0, c1);
+#pragma unroll
+      for (int c = 0; c < L; ++c) if (c * LATE / L == l) load(cur, c, p, p2, q, far, w);
+#pragma unroll
+      for (int i = 0; i < IP; ++i) acc[i][(N - LATE + l) % IQ] = mma<T>(H == 2 ? last[i] : first[i], qf[N - LATE + l], acc[i][(N - LATE + l) % IQ]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -199,18 +248,17 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
   typedef Tile<T, O, BP, BQ, WP, WQ, EPI, DP, DQ> K;
   constexpr bool GATED = EPI == EPI_GATED;
   constexpr int COLS = GATED ? BP / 2 : BP, NT = WP * WQ * 64;
-  __shared__ __attribute__((aligned(1024))) char stage[2 * K::STAGE];
-  lds_t* s0 = (lds_t*)stage;
-  lds_t* s1 = s0 + K::STAGE;
+  __shared__ __attribute__((aligned(1024))) char stage[K::LDS];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = w % WP, wq = w / WP;
   int tp, tq;
   tile_of(blockIdx.x, a.tiles_p, a.tiles_q, tp, tq);
   const int n0 = tp * COLS, m0 = tq * BQ;
-  const int per = (a.ksteps + a.splits - 1) / a.splits, k0 = blockIdx.y * per, k1 = min(a.ksteps, k0 + per);      // this split's stages
+  const int stages = DP ? (a.krows + K::P::RK - 1) / K::P::RK : (a.kbytes + K::SB - 1) / K::SB;
+  const int per = (stages + a.splits - 1) / a.splits, k0 = blockIdx.y * per, k1 = min(stages, k0 + per);      // this split's stages
 
   K t;
   // first elements of the tile's operands at stage k0, and how far a stage moves them
-  const int64_t dp = DP ? K::P::RK * a.ldp : 128, dq = DQ ? K::Q::RK * a.ldq : 128;
+  const int64_t dp = DP ? K::P::RK * a.ldp : K::SB, dq = DQ ? K::Q::RK * a.ldq : K::SB;
   const int second = min(n0 + BP / 2, a.np - 1);      // (not gated, K along rows: the tile's other half of rows)
   const char* p = a.p + (DP ? (int64_t)n0 * K::P::ES : (int64_t)n0 * a.ldp) + k0 * dp;
   const char* p2 = (GATED ? a.p2 + (int64_t)n0 * a.ldp : a.p + (int64_t)second * a.ldp) + k0 * dp;
@@ -221,8 +269,8 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
 #pragma unroll
   for (int c = 0; c < K::LP; ++c) {
     const int at = c * K::NW * 1024 + mine;
-    const bool upper = !DP && c * K::NW * 1024 >= BP * 64;
-    t.po[c] = K::P::source(upper ? at - BP * 64 : at, a.ldp, a.np - 1 - (upper && !GATED ? second : n0), (a.np - n0) * K::P::ES);
+    const bool upper = !DP && c * K::NW * 1024 >= BP / 2 * K::SB;
+    t.po[c] = K::P::source(upper ? at - BP / 2 * K::SB : at, a.ldp, a.np - 1 - (upper && !GATED ? second : n0), (a.np - n0) * K::P::ES);
   }
 #pragma unroll
   for (int c = 0; c < K::LQ; ++c) t.qo[c] = K::Q::source(c * K::NW * 1024 + mine, a.ldq, a.nq - 1 - m0, (a.nq - m0) * K::Q::ES);
@@ -231,21 +279,30 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
     t.pa[i] = K::P::place(GATED ? (i < K::IP / 2 ? wp * (K::IP / 2) + i : BP / 32 + wp * (K::IP / 2) + i - K::IP / 2) : wp * K::IP + i, lane);
 #pragma unroll
   for (int j = 0; j < K::IQ; ++j) t.qa[j] = K::Q::place(wq * K::IQ + j, lane);
-  const int c0 = ((lane >> 4) ^ (lane & 7)) * 16, c1 = ((4 + (lane >> 4)) ^ (lane & 7)) * 16;
+  const int turn = K::SB == 64 ? (lane >> 2) & 3 : lane & 7, c0 = ((lane >> 4) ^ turn) * 16, c1 = ((4 + (lane >> 4)) ^ turn) * 16;
 #pragma unroll
   for (int i = 0; i < K::IP; ++i)
 #pragma unroll
     for (int j = 0; j < K::IQ; ++j) t.acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  if (k0 < k1) t.fill(s0, a, p, p2, q, k0, w);
-  for (int k = k0; k < k1; ++k) {
-    p += dp; p2 += dp; q += dq;
-    __builtin_amdgcn_s_waitcnt(0x0f70);      // this wave's loads have reached LDS (issued a whole stage ago) ...
-    __syncthreads();                         // ... and so have the others'; and everyone is done with the other stage
-    t.step(s0, s1, a, p, p2, q, k + 1, k + 1 < k1, w, c0, c1);
-    lds_t* x = s0; s0 = s1; s1 = x;
+  t.ends_p = DP ? min(a.krows, k1 * K::P::RK) : min(a.kbytes, k1 * K::SB);
+  t.ends_q = DQ ? min(a.krows, k1 * K::Q::RK) : min(a.kbytes, k1 * K::SB);
+  typename K::part pf[2][K::IP], ahead[K::LATE];
+  lds_t* cur = (lds_t*)stage;
+  lds_t* const stop = cur + K::LDS;
+  t.begin(cur, cur + K::STAGE, pf[0], ahead, p, p2, q, dp, dq, k0, w, c0, c1);
+  p += K::NS * dp; p2 += K::NS * dp; q += K::NS * dq;
+  for (int k = k0; k < k1; k += 2) {         // two stages a turn, each with registers of its own for p (an odd number of stages ends with one of zeros)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      lds_t* const nxt = cur + K::STAGE == stop ? (lds_t*)stage : cur + K::STAGE;
+      t.step(cur, nxt, pf[h], pf[1 - h], ahead, p, p2, q, k + h + K::NS, w, c0, c1);
+      p += dp; p2 += dp; q += dq;
+      cur = nxt;
+    }
   }
-  __syncthreads();                           // the stages are free for the results
+  // the last loads (zeros) and reads have ended: the stages are free for the results
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
   // a lane holds columns 4 (lane / 16) .. + 3 of row lane % 16 of each 16 x 16 block
   lds_t* const out = (lds_t*)stage;
@@ -272,10 +329,10 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
   }
   typedef O o4 __attribute__((ext_vector_type(4)));
   if constexpr (!GATED) {
-    // in as many turns over the tile's rows as its results are larger than the two stages
-    constexpr int TURNS = (BQ * COLS * (int)sizeof(O) + 2 * K::STAGE - 1) / (2 * K::STAGE), R = BQ / TURNS;
+    // in as many turns over the tile's rows as its results are larger than the stages
+    constexpr int TURNS = (BQ * COLS * (int)sizeof(O) + K::LDS - 1) / K::LDS, R = BQ / TURNS;
     typedef Out<O, R, COLS, NT> Z;
-    static_assert(Z::BYTES <= 2 * K::STAGE && (TURNS == 1 || TURNS == WQ), "a turn: the rows of one row of waves");
+    static_assert(Z::BYTES <= K::LDS && (TURNS == 1 || TURNS == WQ), "a turn: the rows of one row of waves");
     O* base = static_cast<O*>(a.out) + (int64_t)m0 * a.ldo + n0;
 #pragma unroll
     for (int turn = 0; turn < TURNS; ++turn) {
@@ -310,7 +367,7 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
       }
     }
     typedef Out<O, BQ, COLS, NT> Z;
-    static_assert(Z::BYTES <= 2 * K::STAGE, "the results fit the stages");
+    static_assert(Z::BYTES <= K::LDS, "the results fit the stages");
     auto put_out = [&](auto act) {
 #pragma unroll
       for (int j = 0; j < K::IQ; ++j)
@@ -343,8 +400,8 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
       uint16_t* saved = static_cast<uint16_t*>(a.saved) + first;
 #pragma unroll
       for (int h = 0; h < 3; ++h) {            // two places in turn: one barrier a plane
-        lds_t* const at = 2 * S::BYTES <= 2 * K::STAGE ? out + (h & 1 ? 0 : S::BYTES) : out;
-        if (2 * S::BYTES > 2 * K::STAGE) __syncthreads();
+        lds_t* const at = 2 * S::BYTES <= K::LDS ? out + (h & 1 ? 0 : S::BYTES) : out;
+        if (2 * S::BYTES > K::LDS) __syncthreads();
 #pragma unroll
         for (int j = 0; j < K::IQ; ++j)
 #pragma unroll
@@ -418,6 +475,21 @@ __device__ __forceinline__ i32x4 chunk_at(const char* row, int64_t at, int64_t k
   for (int i = 0; i < 16; ++i) if (at + i < kbytes) u.b[i] = row[at + i];
   return u.v;
 }
+template <class T, bool WHOLE> __device__ __forceinline__ void few_step(const char* pg, const char* pu, const char* const* q, int mq, int64_t c0, int64_t c1, int64_t kbytes, f32x4* g, f32x4* u) {
+  auto at = [&](const char* row, int64_t c) { return WHOLE ? __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(row + c)) : chunk_at(row, c, kbytes); };
+  const i32x4 x0 = at(pg, c0), x1 = at(pg, c1), y0 = at(pu, c0), y1 = at(pu, c1);
+#pragma unroll
+  for (int j = 0; j < mq; ++j) {
+    const i32x4 z0 = at(q[j], c0), z1 = at(q[j], c1);
+    if constexpr (Piece<T>::count == 2) {
+      g[j] = mma<T>(x1, z1, mma<T>(x0, z0, g[j]));
+      u[j] = mma<T>(y1, z1, mma<T>(y0, z0, u[j]));
+    } else {
+      g[j] = mma<T>(join(x0, x1), join(z0, z1), g[j]);
+      u[j] = mma<T>(join(y0, y1), join(z0, z1), u[j]);
+    }
+  }
+}
 template <class T, class O, int MQ> __global__ __launch_bounds__(1024) void k_few_rows(Product a) {
   __shared__ f32x4 part[15 * 64 * 2 * MQ];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
@@ -425,35 +497,16 @@ template <class T, class O, int MQ> __global__ __launch_bounds__(1024) void k_fe
   const char* pg = a.p + (int64_t)row * a.ldp;
   const char* pu = a.p2 + (int64_t)row * a.ldp;
   const char* q[MQ];
-#pragma unroll
-  for (int j = 0; j < MQ; ++j) q[j] = a.q + (int64_t)min(j * 16 + (lane & 15), a.nq - 1) * a.ldq;
   f32x4 g[MQ], u[MQ];
 #pragma unroll
-  for (int j = 0; j < MQ; ++j) g[j] = u[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < MQ; ++j) {
+    q[j] = a.q + (int64_t)min(j * 16 + (lane & 15), a.nq - 1) * a.ldq;
+    g[j] = u[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   const int whole = a.kbytes / 128;
   const int64_t c0 = (lane >> 4) * 16, c1 = c0 + 64;
-  for (int k = w; k < whole; k += nw) {
-    const int64_t at = (int64_t)k * 128;
-    i32x4 x[2] = {__builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(pg + at + c0)), __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(pg + at + c1))};
-    i32x4 y[2] = {__builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(pu + at + c0)), __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(pu + at + c1))};
-#pragma unroll
-    for (int j = 0; j < MQ; ++j) {
-      const i32x4 z[2] = {__builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(q[j] + at + c0)), __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(q[j] + at + c1))};
-      g[j] = mma<T>(x, z, g[j]);
-      u[j] = mma<T>(y, z, u[j]);
-    }
-  }
-  if (whole * 128 < a.kbytes && whole % nw == w) {
-    const int64_t at = (int64_t)whole * 128;
-    const i32x4 x[2] = {chunk_at(pg, at + c0, a.kbytes), chunk_at(pg, at + c1, a.kbytes)};
-    const i32x4 y[2] = {chunk_at(pu, at + c0, a.kbytes), chunk_at(pu, at + c1, a.kbytes)};
-#pragma unroll
-    for (int j = 0; j < MQ; ++j) {
-      const i32x4 z[2] = {chunk_at(q[j], at + c0, a.kbytes), chunk_at(q[j], at + c1, a.kbytes)};
-      g[j] = mma<T>(x, z, g[j]);
-      u[j] = mma<T>(y, z, u[j]);
-    }
-  }
+  for (int k = w; k < whole; k += nw) few_step<T, true>(pg, pu, q, MQ, k * 128ll + c0, k * 128ll + c1, a.kbytes, g, u);
+  if (whole * 128 < a.kbytes && whole % nw == w) few_step<T, false>(pg, pu, q, MQ, whole * 128ll + c0, whole * 128ll + c1, a.kbytes, g, u);
   if (w > 0) {
 #pragma unroll
     for (int j = 0; j < MQ; ++j) {
@@ -572,7 +625,7 @@ int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
 struct Plan { int bp, bq, splits; };      // bp = 0: the kernel for few rows (bq rows a workgroup)
 
-// Tile and K split of a product with `cols` columns (of 2 `cols` rows of p when gated), `rows` rows and K of `ksteps` stages.
+// Tile and K split of a product with `cols` columns (of 2 `cols` rows of p when gated), `rows` rows and K of `ksteps` times 128 bytes.
 Plan plan_of(bool gated, int64_t rows, int64_t cols, int ksteps) {
   Plan p;
   const int64_t prows = gated ? 2 * cols : cols;
@@ -581,7 +634,7 @@ Plan plan_of(bool gated, int64_t rows, int64_t cols, int ksteps) {
   p = {128, rows <= 32 ? 32 : rows <= 64 ? 64 : 128, 1};
   const int64_t w = wgs(p.bp, p.bq);
   int64_t s = w >= 256 ? 1 : (512 + w - 1) / w;
-  if (s > ksteps / 4) s = ksteps / 4;      // at least 4 stages a piece
+  if (s > ksteps / 4) s = ksteps / 4;      // at least 512 bytes of K a piece
   if (s > 16) s = 16;
   p.splits = s < 1 ? 1 : (int)s;
   return p;
@@ -591,8 +644,7 @@ template <class T, class O, int EPI, bool DP = false, bool DQ = false> int launc
   const int cols = EPI == EPI_GATED ? p.bp / 2 : p.bp;
   a.tiles_p = cdiv(a.np, cols);
   a.tiles_q = cdiv(a.nq, p.bq);
-  const int per = cdiv(a.ksteps, p.splits);
-  a.splits = cdiv(a.ksteps, per);          // no empty piece
+  a.splits = p.splits;
   const dim3 grid((unsigned)(a.tiles_p * a.tiles_q), (unsigned)a.splits);
   if (p.bp == 256) hipLaunchKernelGGL((k_product<T, O, 256, 256, 4, 2, EPI, DP, DQ>), grid, dim3(512), 0, st, a);
   else if (p.bq == 128) hipLaunchKernelGGL((k_product<T, O, 128, 128, 2, 2, EPI, DP, DQ>), grid, dim3(256), 0, st, a);
@@ -636,7 +688,7 @@ int pad_rows(void* dst, const void* src, int64_t rows, int64_t kbytes, int64_t l
 template <class T, class O> int few_rows(Product& a, hipStream_t st, const char* what) {
   const int blocks = cdiv(a.np, 16);
   int nw = 4;                              // waves that share K: more where there are few workgroups, at least 2 stages each
-  while (nw < 16 && blocks * nw < 4096 && a.ksteps >= 4 * nw) nw *= 2;
+  while (nw < 16 && blocks * nw < 4096 && a.kbytes >= 512 * nw) nw *= 2;
   if (a.nq <= 16) hipLaunchKernelGGL((k_few_rows<T, O, 1>), dim3(blocks), dim3(nw * 64), 0, st, a);
   else hipLaunchKernelGGL((k_few_rows<T, O, 2>), dim3(blocks), dim3(nw * 64), 0, st, a);
   return check_launch(what);
@@ -677,7 +729,7 @@ BwdLayout bwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, i
 
 template <class T> int backward(void* dx, void* dw, void* db, char* ws, const void* dy, const void* saved, const void* x, const void* w, int64_t rows, int64_t n,
                                 int64_t k, int64_t ldx, int64_t ldw, int64_t lddy, int dtype, int act, float scale, hipStream_t st, const char* what) {
-  const int e = sizeof(T), v = 16 / e, rk = 128 / e;
+  const int e = sizeof(T), v = 16 / e;
   const bool x_ok = !dw || aligned(x, ldx * e, k * e), w_ok = !dx || aligned(w, ldw * e, k * e);
   const BwdLayout l = bwd_layout(rows, n, k, x_ok, w_ok, dtype, dx != nullptr, dw != nullptr, db != nullptr);
   T* z = dx || dw ? (T*)(ws + l.z) : nullptr;
@@ -700,7 +752,7 @@ template <class T> int backward(void* dx, void* dw, void* db, char* ws, const vo
     a.p = (const char*)w; a.ldp = ldw * e;
     if (!w_ok) { if ((rc = pad_rows(ws + l.wpad, w, 2 * n, k * e, ldw * e, st, what)) != CAGC_OK) return rc; a.p = ws + l.wpad; a.ldp = l.kpad; }
     a.nq = (int)rows;
-    a.kbytes = (int)(l.ldz * e); a.krows = (int)(2 * n); a.ksteps = cdiv(2 * n, rk);
+    a.kbytes = (int)(l.ldz * e); a.krows = (int)(2 * n);
     a.out = dx;
     if ((rc = launch_product<T, T, EPI_PLAIN, true, false>(a, l.dx, st, what)) != CAGC_OK) return rc;
   }
@@ -708,7 +760,7 @@ template <class T> int backward(void* dx, void* dw, void* db, char* ws, const vo
     a.p = (const char*)x; a.ldp = ldx * e;
     if (!x_ok) { if ((rc = pad_rows(ws + l.xpad, x, rows, k * e, ldx * e, st, what)) != CAGC_OK) return rc; a.p = ws + l.xpad; a.ldp = l.kpad; }
     a.nq = (int)(2 * n);
-    a.kbytes = 0; a.krows = (int)rows; a.ksteps = cdiv(rows, rk);
+    a.kbytes = 0; a.krows = (int)rows;
     a.out = dw;
     if ((rc = launch_product<T, T, EPI_PLAIN, true, true>(a, l.dw, st, what)) != CAGC_OK) return rc;
   }
@@ -748,7 +800,7 @@ extern "C" int cagc_gated_linear_fwd(void* out, void* saved, void* ws, const voi
   a.p = (const char*)w; a.ldp = ldw * e;
   a.q = (const char*)x; a.ldq = ldx * e;
   a.np = (int)n; a.nq = (int)rows;
-  a.kbytes = (int)kb; a.ksteps = cdiv(kb, 128);
+  a.kbytes = (int)kb;
   a.out = out; a.ldo = n;
   a.alpha = scale; a.bias = bias; a.sp = w_scale; a.sq = x_scale; a.saved = saved; a.act = act;
   a.splits = 1;

@@ -182,14 +182,30 @@ ROW_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 3, torch.float8
 
 
 def rows_of(t, width):
-    """`t` [..., width] as rows for the row-wise entry points: (tensor [rows, width] with unit stride along a row, elements from row to
-    row).  A view where the strides allow it, else a copy."""
-    r = t.reshape(-1, width) if t.dim() != 2 else t
+    """`t` [..., width] as rows for the row-wise entry points: (tensor that holds them, number of rows, elements from row to row).  The tensor
+    itself where its strides allow that, else a copy."""
+    if t.is_contiguous():
+        return t, t.numel() // width, width
+    r = t.reshape(-1, width)
     n, s = r.shape[0], r.stride(0)
     if (width > 1 and r.stride(1) != 1) or (n > 1 and s < width):
-        r = r.contiguous()
-        s = width
-    return r, (s if n > 1 else width)
+        r, s = r.contiguous(), width
+    return r, n, (s if n > 1 else width)
+
+
+def address(t):
+    return None if t is None else t.data_ptr()
+
+
+def launch(name, device, *args):
+    """`call` on the current stream of device number `device`"""
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return call(name, *args)
+    lib = _lib if _lib is not None else load()
+    rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc != 0:
+        raise RuntimeError(f"{name} failed ({rc}): {lib.cagc_last_error().decode()}")
 
 
 def ptr_any(t):
@@ -201,7 +217,8 @@ def ptr_any(t):
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    """the current stream of the current device, as the address that the library takes"""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def call(name, *args):

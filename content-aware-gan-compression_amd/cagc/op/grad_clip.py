@@ -4,29 +4,30 @@
 GPU tensors -> cagc_clip_grad_norm (csrc/gradnorm.hip): a launch for up to 120 tensors' norm, one that joins it, one that scales (and
 leaves at once where nothing is to be clipped); sums in 64 bits and in a fixed order; nothing waits for the host, so it can be captured.  CPU tensors ->
 composed PyTorch."""
-import ctypes
+from array import array
+from operator import attrgetter
 
 import torch
 
 from .. import _lib
 
 _NORMS = {1.0: 1, 2.0: 2, float("inf"): 0}
+_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 3}
+_T = torch.Tensor
+_dtype, _layout = attrgetter("dtype"), attrgetter("layout")
 
 
-def _tensors(name, tensors):
-    """the list's tensors, on one device and of types the kernels take"""
-    dev = tensors[0].device
-    for t in tensors:
-        if t.device != dev or t.layout != torch.strided or (dev.type != "cpu" and t.dtype not in _lib.ROW_DTYPE or t.dtype == torch.float8_e4m3fn):
-            raise RuntimeError(f"{name}: {t.dtype} {t.layout} tensor on {t.device} (dense fp32 / fp16 / bf16 gradients on one device)")
-    return dev
-
-
-def _norm_code(name, norm_type):
+def _check(name, tensors, norm_type):
+    """(number of the device that all the tensors are on, the norm's code)"""
     code = _NORMS.get(float(norm_type))
     if code is None:
         raise RuntimeError(f"{name}: norm_type {norm_type} (1, 2 or inf)")
-    return code
+    devices, dtypes, layouts = set(map(_T.get_device, tensors)), set(map(_dtype, tensors)), set(map(_layout, tensors))
+    dev = tensors[0].get_device()
+    if len(devices) > 1 or layouts != {torch.strided} or (dev >= 0 and not dtypes <= _CODES.keys()) or not all(t.is_floating_point for t in dtypes):
+        raise RuntimeError(f"{name}: tensors of {sorted(map(str, dtypes))} {sorted(map(str, layouts))} on devices {sorted(devices)} "
+                           "(dense fp32 / fp16 / bf16 gradients on one device)")
+    return dev, code
 
 
 def _composed_norm(tensors, code):
@@ -38,19 +39,21 @@ def _composed_norm(tensors, code):
 
 def _launch(tensors, code, max_norm, scale, dev):
     """the norm (0-dim fp32); with `scale`, the tensors are clipped in place"""
-    flat = [t if t.is_contiguous() else t.contiguous() for t in tensors]
-    n = len(flat)
-    p = (ctypes.c_void_p * n)(*[t.data_ptr() for t in flat])
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in flat])
-    types = (ctypes.c_int * n)(*[_lib.ROW_DTYPE[t.dtype] for t in flat])
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = torch.empty(_lib.query("cagc_grad_norm_workspace", sizes, n), dtype=torch.uint8, device=dev)
-    with _lib.on_device(norm):
-        _lib.call("cagc_clip_grad_norm", norm.data_ptr(), ws.data_ptr(), p, sizes, types, n, code, max_norm, scale)
+    flat, n = tensors, len(tensors)
+    if not all(map(_T.is_contiguous, tensors)):
+        flat = [t.contiguous() for t in tensors]
+    p, sizes = array("Q", map(_T.data_ptr, flat)), array("q", map(_T.numel, flat))
+    types = array("i", map(_CODES.__getitem__, map(_dtype, flat)))
+    sizes_at = sizes.buffer_info()[0]
+    norm = flat[0].new_empty((), dtype=torch.float32)
+    ws = norm.new_empty(_lib.query("cagc_grad_norm_workspace", sizes_at, n) // 4)
+    _lib.launch("cagc_clip_grad_norm", dev, norm.data_ptr(), ws.data_ptr(), p.buffer_info()[0], sizes_at, types.buffer_info()[0], n, code, max_norm, scale)
     if scale:
-        for t, f in zip(tensors, flat):
-            if f is not t:
-                t.copy_(f)
+        if flat is not tensors:
+            with torch.no_grad():
+                for t, f in zip(tensors, flat):
+                    if f is not t:
+                        t.copy_(f)
         torch.autograd.graph.increment_version(tensors)
     return norm
 
@@ -60,36 +63,38 @@ def _finite(name, norm, error_if_nonfinite):
         raise RuntimeError(f"{name}: the norm of the gradients is not finite")
 
 
-@torch.no_grad()
 def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False):
-    """Norm of all the tensors' elements together (0-dim fp32 on their device)."""
+    """Norm of all the tensors' elements together (0-dim fp32 on their device; not differentiated)."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    code = _norm_code("get_total_norm", norm_type)
     if not tensors:
         return torch.tensor(0.0)
-    dev = _tensors("get_total_norm", tensors)
-    norm = _composed_norm(tensors, code).float() if dev.type == "cpu" else _launch(tensors, code, 0.0, 0, dev)
+    dev, code = _check("get_total_norm", tensors, norm_type)
+    if dev < 0:
+        with torch.no_grad():
+            norm = _composed_norm(tensors, code).float()
+    else:
+        norm = _launch(tensors, code, 0.0, 0, dev)
     _finite("get_total_norm", norm, error_if_nonfinite)
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm taken over all of them together, and returns the
     norm before (0-dim fp32 on their device).  error_if_nonfinite waits for the norm and raises before anything is scaled."""
     name = "clip_grad_norm_"
     parameters = [parameters] if torch.is_tensor(parameters) else parameters
-    grads = [p.grad for p in parameters if p.grad is not None]
-    max_norm, code = float(max_norm), _norm_code(name, norm_type)
+    grads = [g for p in parameters if (g := p.grad) is not None]
     if not grads:
         return torch.tensor(0.0)
-    dev = _tensors(name, grads)
-    if dev.type == "cpu":
-        norm = _composed_norm(grads, code)
-        _finite(name, norm, error_if_nonfinite)
-        coef = (max_norm / (norm + 1e-6)).clamp(max=1.0)
-        for g in grads:
-            g.copy_(g * coef if g.dtype == torch.float64 else g.float() * coef.float())
+    max_norm = float(max_norm)
+    dev, code = _check(name, grads, norm_type)
+    if dev < 0:
+        with torch.no_grad():
+            norm = _composed_norm(grads, code)
+            _finite(name, norm, error_if_nonfinite)
+            coef = (max_norm / (norm + 1e-6)).clamp(max=1.0)
+            for g in grads:
+                g.copy_(g * coef if g.dtype == torch.float64 else g.float() * coef.float())
         return norm.float()
     if error_if_nonfinite:
         _finite(name, _launch(grads, code, 0.0, 0, dev), True)

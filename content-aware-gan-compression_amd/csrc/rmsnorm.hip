@@ -142,6 +142,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(Norm a) {
 struct NormBwd {
   void* dx;              // [rows, dim]
   float* part;           // [gridDim.x][dim]: each workgroup's share of dw [nullable]
+  void* dw;              // [dim], of a workgroup that is the only one [nullable]
   const void* dy;
   const void* dh;        // [nullable]
   const void* h;
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm_bwd(NormBwd 
       store_v<V>(dx + (t + c * TPR) * V, d[c], a.dim - (t + c * TPR) * V);
     }
   }
-  if (!a.part) return;
+  if (!a.part && !a.dw) return;
   if (RPB > 1) {                               // the workgroup's rows at once, joined in order
     for (int k = RPB - 1; k > 0; --k) {
       if (slot == k) {
@@ -229,11 +230,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm_bwd(NormBwd 
     }
     if (slot > 0) return;
   }
-  float* part = a.part + (int64_t)blockIdx.x * a.dim;
+  float* part = a.part ? a.part + (int64_t)blockIdx.x * a.dim : nullptr;
 #pragma unroll
   for (int c = 0; c < NV; ++c)
 #pragma unroll
-    for (int i = 0; i < V; ++i) if ((t + c * TPR) * V + i < a.dim) part[(t + c * TPR) * V + i] = dw[c][i];
+    for (int i = 0; i < V; ++i) {
+      const int at = (t + c * TPR) * V + i;
+      if (at >= a.dim) continue;
+      if (part) part[at] = dw[c][i];
+      else static_cast<W*>(a.dw)[at] = (W)dw[c][i];
+    }
 }
 
 // dw[c] = sum of the workgroups' shares, in a fixed order
@@ -281,11 +287,12 @@ template <int OUT> int launch_norm_as(const Norm& a, int dtype, int wdtype, hipS
   return wdtype == CAGC_F32 ? launch_norm<__bf16, float, OUT>(a, st, what) : launch_norm<__bf16, __bf16, OUT>(a, st, what);
 }
 
-// workgroups of a backward: each writes dim floats for dw, so few enough that these stay small beside the rows, enough to fill 256 CUs
+// workgroups of a backward: each writes dim floats for dw, so few enough that these stay small beside the rows, enough to fill 256 CUs; up to four turns of rows
+// are left to one workgroup, which then writes dw itself (16 rows of 512: one launch instead of two, and no workspace)
 int bwd_wgs(int64_t rows, int chunks) {
   const int rpb = chunks <= 128 ? 4 : 1;
   const int64_t need = (rows + rpb - 1) / rpb;
-  return (int)(need < 1024 ? need : 1024);
+  return (int)(need <= 4 ? 1 : need < 1024 ? need : 1024);
 }
 
 template <class T, class W> int launch_bwd(const NormBwd& a, void* dw, hipStream_t st, const char* what) {
@@ -294,7 +301,7 @@ template <class T, class W> int launch_bwd(const NormBwd& a, void* dw, hipStream
   CAGC_ROW_SHAPES(chunks, CAGC_CALL)
 #undef CAGC_CALL
   int rc = check_launch(what);
-  if (rc != CAGC_OK || !dw) return rc;
+  if (rc != CAGC_OK || !a.part) return rc;
   hipLaunchKernelGGL((k_rms_norm_dw<W>), dim3((a.dim + 63) / 64), dim3(1024), 0, st, static_cast<W*>(dw), a.part, wgs, a.dim);
   return check_launch(what);
 }
@@ -338,7 +345,8 @@ extern "C" int cagc_quantize_rows_e4m3(void* q, float* scale, const void* x, int
 }
 extern "C" int64_t cagc_rms_norm_bwd_workspace(int64_t rows, int64_t dim, int dtype) {
   if (rows <= 0 || !row_type(dtype) || !dim_ok(dim, dtype)) return 0;
-  return 4 * dim * bwd_wgs(rows, chunks_of(dim, dtype));
+  const int wgs = bwd_wgs(rows, chunks_of(dim, dtype));
+  return wgs > 1 ? 4 * dim * wgs : 0;
 }
 extern "C" int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, const void* dh, const void* h, const void* w, const float* rstd, int64_t rows,
                                  int64_t dim, int64_t dy_stride, int64_t dh_stride, int64_t h_stride, int dtype, int wdtype, cagc_stream_t stream) {
@@ -346,8 +354,9 @@ extern "C" int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, c
   CAGC_NORM_CHECKS(what);
   CAGC_REQUIRE(rows > 0, "%s: no rows (the weight's gradient is zero)", what);
   if (!dx && !dw) return CAGC_OK;
-  CAGC_REQUIRE(dy && h && rstd && (!dw || ws), "%s: null pointer", what);
-  const NormBwd a = {dx, dw ? static_cast<float*>(ws) : nullptr, dy, dh, h, w, rstd, rows, dy_stride, dh_stride, h_stride, (int)dim};
+  const bool alone = bwd_wgs(rows, chunks_of(dim, dtype)) == 1;
+  CAGC_REQUIRE(dy && h && rstd && (!dw || alone || ws), "%s: null pointer", what);
+  const NormBwd a = {dx, dw && !alone ? static_cast<float*>(ws) : nullptr, alone ? dw : nullptr, dy, dh, h, w, rstd, rows, dy_stride, dh_stride, h_stride, (int)dim};
   hipStream_t st = as_stream(stream);
   if (dtype == CAGC_F32) return launch_bwd<float, float>(a, dw, st, what);
   if (dtype == CAGC_F16) return wdtype == CAGC_F32 ? launch_bwd<_Float16, float>(a, dw, st, what) : launch_bwd<_Float16, _Float16>(a, dw, st, what);

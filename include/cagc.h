@@ -545,7 +545,7 @@ int cagc_rms_norm_e4m3(void* q, float* scale, void* h, const void* x, const void
 /* rows as they are -> e4m3 and a scale per row (weights, once) */
 int cagc_quantize_rows_e4m3(void* q, float* scale, const void* x, int64_t rows, int64_t dim, int64_t x_stride, int dtype, cagc_stream_t stream);
 /* dx [rows, dim] (contiguous; also the residual's gradient) and dw [dim] in wdtype, each nullable; dh [nullable]: the gradient of h from its other use;
- * dy, dh, h: rows dy_stride, dh_stride, h_stride apart.  rows > 0.  ws: cagc_rms_norm_bwd_workspace bytes (only with dw).  Fixed order of summation. */
+ * dy, dh, h: rows dy_stride, dh_stride, h_stride apart.  rows > 0.  ws: cagc_rms_norm_bwd_workspace bytes (only with dw; 0: may be null).  Fixed order of summation. */
 int64_t cagc_rms_norm_bwd_workspace(int64_t rows, int64_t dim, int dtype);
 int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, const void* dh, const void* h, const void* w, const float* rstd, int64_t rows,
                       int64_t dim, int64_t dy_stride, int64_t dh_stride, int64_t h_stride, int dtype, int wdtype, cagc_stream_t stream);

@@ -466,78 +466,113 @@ template <class O, int EPI> __global__ __launch_bounds__(256) void k_join(Produc
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------------------------
-// Up to 16 MQ rows of x: bound by the weights' bytes, each read once, straight into registers.  A workgroup makes 16 output columns (16 gate
-// and 16 up rows); its waves share out K and are added through LDS.  Rows need no alignment: the loads are 16 bytes from any address.
+// Up to 16 MQ rows of x: bound by the weights' bytes, each read once, straight into registers.  A workgroup makes C output columns; its waves share out K, 128 bytes a turn, and are added
+// through LDS.  C = 16: 16 gate rows and 16 up rows, a product for each; C = 8: 8 gate and 8 up rows in ONE product, twice the workgroups: a CU brings in about 40 GB/s whatever its
+// waves have on the way (more turns' loads at once changed nothing), so where there are fewer workgroups than CUs their number decides.
+// Rows need no alignment: the loads are 16 bytes from any address.
+__device__ __forceinline__ i32x4 load16(const char* p) { return __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(p)); }
+// chunk of 16 bytes at `at` of a row of kbytes: zero behind its end
 __device__ __forceinline__ i32x4 chunk_at(const char* row, int64_t at, int64_t kbytes) {
-  if (at + 16 <= kbytes) return __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(row + at));
+  if (at + 16 <= kbytes) return load16(row + at);
   union { uint8_t b[16]; i32x4 v; } u;
   u.v = i32x4{0, 0, 0, 0};
   for (int i = 0; i < 16; ++i) if (at + i < kbytes) u.b[i] = row[at + i];
   return u.v;
 }
-template <class T, bool WHOLE> __device__ __forceinline__ void few_step(const char* pg, const char* pu, const char* const* q, int mq, int64_t c0, int64_t c1, int64_t kbytes, f32x4* g, f32x4* u) {
-  auto at = [&](const char* row, int64_t c) { return WHOLE ? __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(row + c)) : chunk_at(row, c, kbytes); };
-  const i32x4 x0 = at(pg, c0), x1 = at(pg, c1), y0 = at(pu, c0), y1 = at(pu, c1);
-#pragma unroll
-  for (int j = 0; j < mq; ++j) {
-    const i32x4 z0 = at(q[j], c0), z1 = at(q[j], c1);
-    if constexpr (Piece<T>::count == 2) {
-      g[j] = mma<T>(x1, z1, mma<T>(x0, z0, g[j]));
-      u[j] = mma<T>(y1, z1, mma<T>(y0, z0, u[j]));
-    } else {
-      g[j] = mma<T>(join(x0, x1), join(z0, z1), g[j]);
-      u[j] = mma<T>(join(y0, y1), join(z0, z1), u[j]);
-    }
-  }
+template <class T> __device__ __forceinline__ f32x4 mma128(const i32x4 (&a)[2], const i32x4 (&b)[2], f32x4 c) {
+  if constexpr (Piece<T>::count == 2) return mma<T>(a[1], b[1], mma<T>(a[0], b[0], c));
+  else return mma<T>(join(a[0], a[1]), join(b[0], b[1]), c);
 }
-template <class T, class O, int MQ> __global__ __launch_bounds__(1024) void k_few_rows(Product a) {
-  __shared__ f32x4 part[15 * 64 * 2 * MQ];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-  const int n0 = blockIdx.x * 16, row = min(n0 + (lane & 15), a.np - 1);
-  const char* pg = a.p + (int64_t)row * a.ldp;
-  const char* pu = a.p2 + (int64_t)row * a.ldp;
+template <class T, class O, int MQ, int C> __global__ __launch_bounds__(1024) void k_few_rows(Product a) {
+  constexpr int P = C / 8;                 // products a turn
+  extern __shared__ f32x4 part[];          // [nw / 2][MQ][P][64]
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, r = lane & 15;
+  const int n0 = blockIdx.x * C, c0 = (lane >> 4) * 16;
+  // this lane's rows
+  const char* row[P];
   const char* q[MQ];
-  f32x4 g[MQ], u[MQ];
 #pragma unroll
-  for (int j = 0; j < MQ; ++j) {
-    q[j] = a.q + (int64_t)min(j * 16 + (lane & 15), a.nq - 1) * a.ldq;
-    g[j] = u[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int i = 0; i < P; ++i) row[i] = ((P == 1 ? r >= 8 : i == 1) ? a.p2 : a.p) + (int64_t)min(n0 + r % C, a.np - 1) * a.ldp + c0;
+#pragma unroll
+  for (int j = 0; j < MQ; ++j) q[j] = a.q + (int64_t)min(j * 16 + r, a.nq - 1) * a.ldq + c0;
+  f32x4 acc[MQ][P];
+#pragma unroll
+  for (int j = 0; j < MQ; ++j)
+#pragma unroll
+    for (int i = 0; i < P; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  i32x4 x[P][2], z[MQ][2];
+  auto mul = [&]() {
+#pragma unroll
+    for (int j = 0; j < MQ; ++j)
+#pragma unroll
+      for (int i = 0; i < P; ++i) acc[j][i] = mma128<T>(x[i], z[j], acc[j][i]);
+  };
   const int whole = a.kbytes / 128;
-  const int64_t c0 = (lane >> 4) * 16, c1 = c0 + 64;
-  for (int k = w; k < whole; k += nw) few_step<T, true>(pg, pu, q, MQ, k * 128ll + c0, k * 128ll + c1, a.kbytes, g, u);
-  if (whole * 128 < a.kbytes && whole % nw == w) few_step<T, false>(pg, pu, q, MQ, whole * 128ll + c0, whole * 128ll + c1, a.kbytes, g, u);
-  if (w > 0) {
+  for (int k = w; k < whole; k += nw) {
 #pragma unroll
-    for (int j = 0; j < MQ; ++j) {
-      part[((w - 1) * 2 * MQ + 2 * j) * 64 + lane] = g[j];
-      part[((w - 1) * 2 * MQ + 2 * j + 1) * 64 + lane] = u[j];
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) x[i][h] = load16(row[i] + k * 128ll + h * 64);
+#pragma unroll
+      for (int j = 0; j < MQ; ++j) z[j][h] = load16(q[j] + k * 128ll + h * 64);
     }
+    mul();
+  }
+  if (whole * 128 < a.kbytes && whole % nw == w) {
+    const int64_t o = whole * 128ll + c0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) x[i][h] = chunk_at(row[i] - c0, o + h * 64, a.kbytes);
+#pragma unroll
+      for (int j = 0; j < MQ; ++j) z[j][h] = chunk_at(q[j] - c0, o + h * 64, a.kbytes);
+    }
+    mul();
+  }
+  for (int half = nw / 2; half > 0; half /= 2) {      // the upper half of the waves hands its sums to the lower
+    if (w >= half && w < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < MQ; ++j)
+#pragma unroll
+        for (int i = 0; i < P; ++i) part[(((w - half) * MQ + j) * P + i) * 64 + lane] = acc[j][i];
+    }
+    __syncthreads();
+    if (w < half) {
+#pragma unroll
+      for (int j = 0; j < MQ; ++j)
+#pragma unroll
+        for (int i = 0; i < P; ++i) acc[j][i] += part[((w * MQ + j) * P + i) * 64 + lane];
+    }
+    __syncthreads();
+  }
+  // the sums once more through LDS: every wave stores some rows, and gate and up meet (C = 8: up is in the upper 32 lanes)
+  if (w == 0) {
+#pragma unroll
+    for (int j = 0; j < MQ; ++j)
+#pragma unroll
+      for (int i = 0; i < P; ++i) part[(j * P + i) * 64 + lane] = acc[j][i];
   }
   __syncthreads();
-  if (w > 0) return;
-  for (int s = 0; s + 1 < nw; ++s)
-#pragma unroll
-    for (int j = 0; j < MQ; ++j) {
-      g[j] += part[(s * 2 * MQ + 2 * j) * 64 + lane];
-      u[j] += part[(s * 2 * MQ + 2 * j + 1) * 64 + lane];
-    }
   const int n = n0 + (lane >> 4) * 4;
-#pragma unroll
-  for (int j = 0; j < MQ; ++j) {
-    const int m = j * 16 + (lane & 15);
-    if (m < a.nq && n < a.np) gated_out<O>(a, m, n, g[j], u[j]);
+  if (P == 1 && lane >= 32) return;
+  for (int j = w; j < MQ; j += nw) {
+    const int m = j * 16 + r;
+    if (m < a.nq && n < a.np) gated_out<O>(a, m, n, part[j * P * 64 + lane], P == 1 ? part[j * 64 + lane + 32] : part[(j * P + 1) * 64 + lane]);
   }
 }
 
 // ---- layout passes ----------------------------------------------------------------------------------------------------------------
-// rows of any stride and alignment -> rows of `width16` chunks of 16 bytes, the rest of the last chunk zero
-__global__ __launch_bounds__(256) void k_pad_rows(char* __restrict__ dst, const char* __restrict__ src, int64_t rows, int64_t kbytes, int64_t ld, int width16) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= rows * width16) return;
-  const int64_t r = id / width16, c = (id % width16) * 16;
-  *reinterpret_cast<i32x4*>(dst + (r * width16 * 16 + c)) = chunk_at(src + r * ld, c, kbytes);
+// rows of any stride and alignment -> rows of whole 16-byte chunks, the rest of the last chunk zero; up to two operands in one launch
+struct Pad { char* dst; const char* src; int64_t rows, kbytes, ld; };
+__global__ __launch_bounds__(256) void k_pad_rows(Pad a, Pad b, int64_t blocks_a) {
+  const bool second = blockIdx.x >= blocks_a;
+  const Pad p = second ? b : a;
+  const int64_t id = (blockIdx.x - (second ? blocks_a : 0)) * 256 + threadIdx.x, width = (p.kbytes + 15) / 16;
+  if (id >= p.rows * width) return;
+  const int64_t r = id / width, c = (id - r * width) * 16;
+  *reinterpret_cast<i32x4*>(p.dst + (r * width * 16 + c)) = chunk_at(p.src + r * p.ld, c, p.kbytes);
 }
+
 // dz [rows, ldz] from the saved pre-activations and dy (zeros behind 2n), 8 or 4 columns a thread (16 bytes of dz), and the column sums of a band of rows
 // for db.  Bound by its bytes: dy, 3 planes of 16 bits (2 of fp32) and dz's two halves.
 constexpr int BAND = 64;      // rows of a workgroup
@@ -659,7 +694,9 @@ template <class T, class O, int EPI, bool DP = false, bool DQ = false> int launc
 // 16-byte alignment of a matrix's rows and row length: what the tiled product's loads want
 bool aligned(const void* p, int64_t ld_bytes, int64_t kbytes) { return ((uintptr_t)p % 16) == 0 && ld_bytes % 16 == 0 && kbytes % 16 == 0; }
 
-constexpr int64_t FEW = 32;               // rows up to which the weights are streamed through registers
+// Rows whose weights are streamed through registers: up to 32; up to 64 where the weights are small (one launch without padding or a join: 64 x 1001 -> 2731 fp16 18 instead of 24 us, 40 x 512 ->
+// 512 6 instead of 8; with 134 MB of weights, 64 x 4096 -> 8192 bf16, 46 instead of 30) and K does not leave a few workgroups with long rows (61 x 3480 -> 78 fp32 59 instead of 31).
+bool few_rows_do(int64_t rows, int64_t n, int64_t kbytes) { return rows <= 32 || (rows <= 64 && 2 * n * kbytes <= (16 << 20) && kbytes <= 8192); }
 constexpr int64_t MOST_LD = 7 << 20;      // 256 rows of a tile stay within 32-bit offsets
 
 struct FwdLayout { bool few; Plan plan; int64_t xpad, wpad, slab, total; int64_t kpad; };
@@ -667,7 +704,7 @@ FwdLayout fwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, i
   FwdLayout l = {};
   const int64_t kb = k * esize(dtype);
   l.kpad = up16(kb);
-  l.few = rows <= FEW;
+  l.few = few_rows_do(rows, n, kb);
   if (l.few) return l;
   l.plan = plan_of(true, rows, n, (int)((l.kpad + 127) / 128));
   int64_t at = 0;
@@ -679,19 +716,26 @@ FwdLayout fwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, i
   return l;
 }
 
-int pad_rows(void* dst, const void* src, int64_t rows, int64_t kbytes, int64_t ld, hipStream_t st, const char* what) {
-  const int64_t w16 = up16(kbytes) / 16, total = rows * w16;
-  hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (char*)dst, (const char*)src, rows, kbytes, ld, (int)w16);
+int pad_rows(const Pad* jobs, int count, hipStream_t st, const char* what) {
+  if (count == 0) return CAGC_OK;
+  auto blocks = [](const Pad& p) { return (p.rows * ((p.kbytes + 15) / 16) + 255) / 256; };
+  const int64_t first = blocks(jobs[0]), both = first + (count > 1 ? blocks(jobs[1]) : 0);
+  hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)both), dim3(256), 0, st, jobs[0], jobs[count - 1], first);
   return check_launch(what);
 }
 
-template <class T, class O> int few_rows(Product& a, hipStream_t st, const char* what) {
-  const int blocks = cdiv(a.np, 16);
-  int nw = 4;                              // waves that share K: more where there are few workgroups, at least 2 stages each
+template <class T, class O, int MQ, int C> int launch_few(Product& a, hipStream_t st, const char* what) {
+  const int blocks = cdiv(a.np, C);
+  int nw = 4;                              // waves that share K: more where there are few workgroups, at least 2 turns each
   while (nw < 16 && blocks * nw < 4096 && a.kbytes >= 512 * nw) nw *= 2;
-  if (a.nq <= 16) hipLaunchKernelGGL((k_few_rows<T, O, 1>), dim3(blocks), dim3(nw * 64), 0, st, a);
-  else hipLaunchKernelGGL((k_few_rows<T, O, 2>), dim3(blocks), dim3(nw * 64), 0, st, a);
+  hipLaunchKernelGGL((k_few_rows<T, O, MQ, C>), dim3(blocks), dim3(nw * 64), (size_t)nw / 2 * MQ * (C / 8) * 64 * sizeof(f32x4), st, a);      // (at most 64 KB)
   return check_launch(what);
+}
+template <class T, class O> int few_rows(Product& a, hipStream_t st, const char* what) {
+  const bool narrow = a.np < 16 * 256;
+  if (a.nq <= 16) return narrow ? launch_few<T, O, 1, 8>(a, st, what) : launch_few<T, O, 1, 16>(a, st, what);
+  if (a.nq <= 32) return narrow ? launch_few<T, O, 2, 8>(a, st, what) : launch_few<T, O, 2, 16>(a, st, what);
+  return narrow ? launch_few<T, O, 4, 8>(a, st, what) : launch_few<T, O, 4, 16>(a, st, what);
 }
 
 template <class T, class O> int forward(Product& a, const FwdLayout& l, hipStream_t st, const char* what) {
@@ -748,17 +792,20 @@ template <class T> int backward(void* dx, void* dw, void* db, char* ws, const vo
   a.ldo = k;
   a.np = (int)k;
   a.q = (const char*)z; a.ldq = l.ldz * e;
+  Pad jobs[2];
+  int count = 0;
+  if (!w_ok) jobs[count++] = Pad{ws + l.wpad, (const char*)w, 2 * n, k * e, ldw * e};
+  if (!x_ok) jobs[count++] = Pad{ws + l.xpad, (const char*)x, rows, k * e, ldx * e};
+  if ((rc = pad_rows(jobs, count, st, what)) != CAGC_OK) return rc;
   if (dx) {                                  // dz [rows, 2n] along its rows, W [2n, k] down its columns
-    a.p = (const char*)w; a.ldp = ldw * e;
-    if (!w_ok) { if ((rc = pad_rows(ws + l.wpad, w, 2 * n, k * e, ldw * e, st, what)) != CAGC_OK) return rc; a.p = ws + l.wpad; a.ldp = l.kpad; }
+    a.p = w_ok ? (const char*)w : ws + l.wpad; a.ldp = w_ok ? ldw * e : l.kpad;
     a.nq = (int)rows;
     a.kbytes = (int)(l.ldz * e); a.krows = (int)(2 * n);
     a.out = dx;
     if ((rc = launch_product<T, T, EPI_PLAIN, true, false>(a, l.dx, st, what)) != CAGC_OK) return rc;
   }
   if (dw) {                                  // dz and x [rows, k] down their columns
-    a.p = (const char*)x; a.ldp = ldx * e;
-    if (!x_ok) { if ((rc = pad_rows(ws + l.xpad, x, rows, k * e, ldx * e, st, what)) != CAGC_OK) return rc; a.p = ws + l.xpad; a.ldp = l.kpad; }
+    a.p = x_ok ? (const char*)x : ws + l.xpad; a.ldp = x_ok ? ldx * e : l.kpad;
     a.nq = (int)(2 * n);
     a.kbytes = 0; a.krows = (int)rows;
     a.out = dw;
@@ -807,8 +854,11 @@ extern "C" int cagc_gated_linear_fwd(void* out, void* saved, void* ws, const voi
   char* base = (char*)ws;
   int rc;
   if (!l.few) {
-    if (!x_ok) { if ((rc = pad_rows(base + l.xpad, x, rows, kb, a.ldq, st, what)) != CAGC_OK) return rc; a.q = base + l.xpad; a.ldq = l.kpad; }
-    if (!w_ok) { if ((rc = pad_rows(base + l.wpad, w, 2 * n, kb, a.ldp, st, what)) != CAGC_OK) return rc; a.p = base + l.wpad; a.ldp = l.kpad; }
+    Pad jobs[2];
+    int count = 0;
+    if (!x_ok) { jobs[count++] = Pad{base + l.xpad, a.q, rows, kb, a.ldq}; a.q = base + l.xpad; a.ldq = l.kpad; }
+    if (!w_ok) { jobs[count++] = Pad{base + l.wpad, a.p, 2 * n, kb, a.ldp}; a.p = base + l.wpad; a.ldp = l.kpad; }
+    if ((rc = pad_rows(jobs, count, st, what)) != CAGC_OK) return rc;
     a.kbytes = (int)l.kpad;
     a.slab = (float*)(base + l.slab);
   }

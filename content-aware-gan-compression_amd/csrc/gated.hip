@@ -638,21 +638,6 @@ template <class T> __global__ __launch_bounds__(256) void k_dz(T* __restrict__ z
     dbpart[(int64_t)blockIdx.y * 2 * n + (i / V) * n + col] = s;
   }
 }
-// db[c] = sum of the bands' shares, in a fixed order
-template <class T> __global__ __launch_bounds__(1024) void k_db(T* __restrict__ db, const float* __restrict__ part, int bands, int cols) {
-  __shared__ float sh[16][64];
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6, c = blockIdx.x * 64 + x;
-  float s = 0.f;
-  if (c < cols)
-#pragma unroll 4
-    for (int b = y; b < bands; b += 16) s += part[(int64_t)b * cols + c];
-  sh[y][x] = s;
-  __syncthreads();
-  if (y || c >= cols) return;
-  for (int i = 1; i < 16; ++i) s += sh[i][x];
-  db[c] = (T)s;
-}
-
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 int esize(int dtype) { return dtype == CAGC_F32 ? 4 : dtype == CAGC_E4M3 ? 1 : 2; }
 int64_t up16(int64_t b) { return (b + 15) / 16 * 16; }
@@ -783,7 +768,7 @@ template <class T> int backward(void* dx, void* dw, void* db, char* ws, const vo
   int rc = check_launch(what);
   if (rc != CAGC_OK) return rc;
   if (db) {
-    hipLaunchKernelGGL((k_db<T>), dim3((unsigned)((2 * n + 63) / 64)), dim3(1024), 0, st, (T*)db, part, bands, (int)(2 * n));
+    hipLaunchKernelGGL((k_column_sums<T>), dim3((unsigned)((2 * n + 15) / 16)), dim3(1024), 0, st, (T*)db, part, bands, (int)(2 * n));
     if ((rc = check_launch(what)) != CAGC_OK) return rc;
   }
   Product a = {};

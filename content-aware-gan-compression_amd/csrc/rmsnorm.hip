@@ -13,7 +13,7 @@ namespace {
 template <class T> struct Row { static constexpr int V = 16 / (int)sizeof(T); };
 
 // V e4m3 bytes
-template <int V> __device__ __forceinline__ void store_q(uint8_t* p, const float (&f)[V], float inv, int64_t left) {
+template <int V> __device__ __forceinline__ void store_q(uint8_t* p, const float (&f)[V], float inv, int n) {
   uint32_t d[V / 4];
 #pragma unroll
   for (int i = 0; i < V / 4; ++i) {
@@ -21,16 +21,29 @@ template <int V> __device__ __forceinline__ void store_q(uint8_t* p, const float
     d[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, v, true);
   }
   struct __attribute__((packed, aligned(1))) Any { uint32_t v[V / 4]; };
-  if (left >= V) {
+  if (n >= V) {
     Any a;
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) a.v[i] = d[i];
     *reinterpret_cast<Any*>(p) = a;
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) if (i < left) p[i] = (uint8_t)(d[i / 4] >> (8 * (i & 3)));
+    for (int i = 0; i < V; ++i) if (i < n) p[i] = (uint8_t)(d[i / 4] >> (8 * (i & 3)));
   }
 }
+
+// A thread's chunk of V elements.  The last chunk of a row whose length is no multiple of V begins V before the row's end: its first `skip` elements are the chunk before's too, which counts them;
+// both store the same values there.  A thread behind the row's end stands at the last chunk and counts nothing (skip = V).  `n`: elements there (V, but in a row shorter than that).
+template <int V> struct Chunk {
+  int at, skip, n;
+  __device__ __forceinline__ Chunk(int chunk, int dim) {
+    const int start = chunk * V;
+    at = max(0, min(start, dim - V));
+    skip = min(V, start - at);
+    n = min(V, dim);
+  }
+  __device__ __forceinline__ bool used() const { return skip < V; }
+};
 
 // sum / largest over the TPR threads of a row; every thread gets it.  `sh`: TPR / 64 words of this row's own, one use a call.
 template <int TPR> __device__ __forceinline__ float row_sum(float v, float* sh) {
@@ -70,10 +83,13 @@ struct Norm {
   float eps;
 };
 
+// threads of a workgroup: several rows of a wave each, or one row
+constexpr int threads_of(int tpr) { return tpr == 64 ? 256 : tpr; }
+
 // OUT: 0 = the element type, 1 = e4m3, 2 = e4m3 of the rows themselves, without the norm
 template <class T, class W, int TPR, int NV, int OUT>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(Norm a) {
-  constexpr int V = Row<T>::V, RPB = TPR < 256 ? 256 / TPR : 1;
+__global__ __launch_bounds__(threads_of(TPR)) void k_rms_norm(Norm a) {
+  constexpr int V = Row<T>::V, RPB = threads_of(TPR) / TPR;
   __shared__ float sh[2][TPR / 64];
   const int t = threadIdx.x % TPR;
   const int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
@@ -83,32 +99,42 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(Norm a) {
   T* h = a.h ? static_cast<T*>(a.h) + r * a.dim : nullptr;
   float v[NV][V], ss = 0.f;
 #pragma unroll
-  for (int c = 0; c < NV; ++c) load_v<V>(v[c], x + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+  for (int c = 0; c < NV; ++c) {
+    const Chunk<V> k(t + c * TPR, a.dim);
+    load_v<V>(v[c], x + k.at, k.n);
+  }
   if (res) {
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
+      const Chunk<V> k(t + c * TPR, a.dim);
       float f[V];
-      load_v<V>(f, res + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+      load_v<V>(f, res + k.at, k.n);
 #pragma unroll
       for (int i = 0; i < V; ++i) v[c][i] = (float)(T)(v[c][i] + f[i]);
     }
   }
   if (h) {
 #pragma unroll
-    for (int c = 0; c < NV; ++c) store_v<V>(h + (t + c * TPR) * V, v[c], a.dim - (t + c * TPR) * V);
+    for (int c = 0; c < NV; ++c) {
+      const Chunk<V> k(t + c * TPR, a.dim);
+      if (k.used()) store_v<V>(h + k.at, v[c], k.n);
+    }
   }
   if (OUT != 2) {
 #pragma unroll
-    for (int c = 0; c < NV; ++c)
+    for (int c = 0; c < NV; ++c) {
+      const Chunk<V> k(t + c * TPR, a.dim);
 #pragma unroll
-      for (int i = 0; i < V; ++i) ss += v[c][i] * v[c][i];
+      for (int i = 0; i < V; ++i) ss += i >= k.skip ? v[c][i] * v[c][i] : 0.f;
+    }
     const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, sh[0]) / (float)a.dim + a.eps);
     if (a.rstd && t == 0) a.rstd[r] = rstd;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       if (a.w) {
+        const Chunk<V> k(t + c * TPR, a.dim);
         float f[V];
-        load_v<V>(f, static_cast<const W*>(a.w) + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+        load_v<V>(f, static_cast<const W*>(a.w) + k.at, k.n);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[c][i] *= rstd * f[i];
       } else {
@@ -120,7 +146,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(Norm a) {
   if (OUT == 0) {
     T* y = static_cast<T*>(a.y) + r * a.dim;
 #pragma unroll
-    for (int c = 0; c < NV; ++c) store_v<V>(y + (t + c * TPR) * V, v[c], a.dim - (t + c * TPR) * V);
+    for (int c = 0; c < NV; ++c) {
+      const Chunk<V> k(t + c * TPR, a.dim);
+      if (k.used()) store_v<V>(y + k.at, v[c], k.n);
+    }
     return;
   }
   uint32_t top = 0;
@@ -136,7 +165,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(Norm a) {
   const float inv = 1.f / scale;
   uint8_t* q = static_cast<uint8_t*>(a.y) + r * a.dim;
 #pragma unroll
-  for (int c = 0; c < NV; ++c) store_q<V>(q + (t + c * TPR) * V, v[c], inv, a.dim - (t + c * TPR) * V);
+  for (int c = 0; c < NV; ++c) {
+    const Chunk<V> k(t + c * TPR, a.dim);
+    if (k.used()) store_q<V>(q + k.at, v[c], inv, k.n);
+  }
 }
 
 struct NormBwd {
@@ -154,15 +186,16 @@ struct NormBwd {
 
 // A workgroup takes rows blockIdx.x * RPB, + gridDim.x * RPB, ...: a thread keeps its columns of w and of dw in registers throughout.
 template <class T, class W, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm_bwd(NormBwd a) {
-  constexpr int V = Row<T>::V, RPB = TPR < 256 ? 256 / TPR : 1;
+__global__ __launch_bounds__(threads_of(TPR)) void k_rms_norm_bwd(NormBwd a) {
+  constexpr int V = Row<T>::V, RPB = threads_of(TPR) / TPR;
   __shared__ float sh[2][TPR / 64];
   __shared__ float join[RPB > 1 ? NV * V * TPR : 1];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   constexpr bool KEEP = NV * V * TPR <= 16384;      // wider rows read w again for each row (it stays in L2) rather than spill
   float w[KEEP ? NV : 1][V], dw[NV][V];
   auto weight = [&](int c, float (&f)[V]) {
-    if (a.w) { load_v<V>(f, static_cast<const W*>(a.w) + (t + c * TPR) * V, a.dim - (t + c * TPR) * V); return; }
+    const Chunk<V> k(t + c * TPR, a.dim);
+    if (a.w) { load_v<V>(f, static_cast<const W*>(a.w) + k.at, k.n); return; }
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = 1.f;
   };
@@ -180,18 +213,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm_bwd(NormBwd 
     float d[NV][V], n[NV][V], s = 0.f;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
-      load_v<V>(d[c], dy + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
-      load_v<V>(n[c], h + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+      const Chunk<V> k(t + c * TPR, a.dim);
+      load_v<V>(d[c], dy + k.at, k.n);
+      load_v<V>(n[c], h + k.at, k.n);
     }
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
+      const Chunk<V> k(t + c * TPR, a.dim);
       if (!KEEP) weight(c, w[0]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         n[c][i] *= rstd;
         dw[c][i] += d[c][i] * n[c][i];
         d[c][i] *= w[KEEP ? c : 0][i];
-        s += d[c][i] * n[c][i];
+        s += i >= k.skip ? d[c][i] * n[c][i] : 0.f;
       }
     }
     s = row_sum<TPR>(s, sh[turn]) / (float)a.dim;      // two places in turn: one barrier a row
@@ -199,15 +234,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm_bwd(NormBwd 
     T* dx = static_cast<T*>(a.dx) + r * a.dim;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
+      const Chunk<V> k(t + c * TPR, a.dim);
 #pragma unroll
       for (int i = 0; i < V; ++i) d[c][i] = rstd * (d[c][i] - n[c][i] * s);
       if (a.dh) {
         float f[V];
-        load_v<V>(f, static_cast<const T*>(a.dh) + r * a.dhs + (t + c * TPR) * V, a.dim - (t + c * TPR) * V);
+        load_v<V>(f, static_cast<const T*>(a.dh) + r * a.dhs + k.at, k.n);
 #pragma unroll
         for (int i = 0; i < V; ++i) d[c][i] += f[i];
       }
-      store_v<V>(dx + (t + c * TPR) * V, d[c], a.dim - (t + c * TPR) * V);
+      if (k.used()) store_v<V>(dx + k.at, d[c], k.n);
     }
   }
   if (!a.part && !a.dw) return;
@@ -232,39 +268,27 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm_bwd(NormBwd 
   }
   float* part = a.part ? a.part + (int64_t)blockIdx.x * a.dim : nullptr;
 #pragma unroll
-  for (int c = 0; c < NV; ++c)
+  for (int c = 0; c < NV; ++c) {
+    const Chunk<V> k(t + c * TPR, a.dim);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int at = (t + c * TPR) * V + i;
-      if (at >= a.dim) continue;
-      if (part) part[at] = dw[c][i];
-      else static_cast<W*>(a.dw)[at] = (W)dw[c][i];
+      if (i < k.skip || i >= k.n) continue;
+      if (part) part[k.at + i] = dw[c][i];
+      else static_cast<W*>(a.dw)[k.at + i] = (W)dw[c][i];
     }
+  }
 }
 
-// dw[c] = sum of the workgroups' shares, in a fixed order
-template <class W> __global__ __launch_bounds__(1024) void k_rms_norm_dw(W* __restrict__ dw, const float* __restrict__ part, int parts, int dim) {
-  __shared__ float sh[16][64];
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6, c = blockIdx.x * 64 + x;
-  float s = 0.f;
-  if (c < dim)
-#pragma unroll 4
-    for (int p = y; p < parts; p += 16) s += part[(int64_t)p * dim + c];
-  sh[y][x] = s;
-  __syncthreads();
-  if (y || c >= dim) return;
-  for (int i = 1; i < 16; ++i) s += sh[i][x];
-  dw[c] = (W)s;
-}
-
-// threads a row and chunks a thread: a wave for up to 128 chunks of 16 bytes (no barrier), then 4 waves, then 16
-#define CAGC_ROW_SHAPES(chunks, CALL)      \
-  if (chunks <= 64) { CALL(64, 1); }       \
-  else if (chunks <= 128) { CALL(64, 2); } \
-  else if (chunks <= 256) { CALL(256, 1); } \
+// Threads a row and chunks a thread: a wave for up to 128 chunks of 16 bytes (no barrier), then mostly two chunks a thread.  Four hold so many registers that few rows are on the way (backward of
+// 4096 x 8192 bf16: 256 threads of four 86 us, 512 of two 66), workgroups of an odd number of waves do not fill the four SIMDs (8191 x 5120: 320 threads of two 115 us, 256 of three 91).
+#define CAGC_ROW_SHAPES(chunks, CALL)       \
+  if (chunks <= 64) { CALL(64, 1); }        \
+  else if (chunks <= 128) { CALL(64, 2); }  \
+  else if (chunks <= 256) { CALL(128, 2); } \
   else if (chunks <= 512) { CALL(256, 2); } \
   else if (chunks <= 768) { CALL(256, 3); } \
-  else if (chunks <= 1024) { CALL(256, 4); } \
+  else if (chunks <= 1024) { CALL(512, 2); } \
+  else if (chunks <= 1536) { CALL(768, 2); } \
   else if (chunks <= 2048) { CALL(1024, 2); } \
   else { CALL(1024, 4); }
 
@@ -276,7 +300,7 @@ bool dim_ok(int64_t dim, int dtype) { return dim > 0 && dim * esize(dtype) <= (i
 
 template <class T, class W, int OUT> int launch_norm(const Norm& a, hipStream_t st, const char* what) {
   const int chunks = (a.dim + Row<T>::V - 1) / Row<T>::V;
-#define CAGC_CALL(TPR, NV) hipLaunchKernelGGL((k_rms_norm<T, W, TPR, NV, OUT>), dim3((unsigned)((a.rows + (TPR < 256 ? 256 / TPR : 1) - 1) / (TPR < 256 ? 256 / TPR : 1))), dim3(TPR < 256 ? 256 : TPR), 0, st, a)
+#define CAGC_CALL(TPR, NV) hipLaunchKernelGGL((k_rms_norm<T, W, TPR, NV, OUT>), dim3((unsigned)((a.rows + threads_of(TPR) / TPR - 1) / (threads_of(TPR) / TPR))), dim3(threads_of(TPR)), 0, st, a)
   CAGC_ROW_SHAPES(chunks, CAGC_CALL)
 #undef CAGC_CALL
   return check_launch(what);
@@ -287,22 +311,27 @@ template <int OUT> int launch_norm_as(const Norm& a, int dtype, int wdtype, hipS
   return wdtype == CAGC_F32 ? launch_norm<__bf16, float, OUT>(a, st, what) : launch_norm<__bf16, __bf16, OUT>(a, st, what);
 }
 
-// workgroups of a backward: each writes dim floats for dw, so few enough that these stay small beside the rows, enough to fill 256 CUs; up to four turns of rows
-// are left to one workgroup, which then writes dw itself (16 rows of 512: one launch instead of two, and no workspace)
-int bwd_wgs(int64_t rows, int chunks) {
+// Workgroups of a backward: at most as many as 256 CUs hold at once (at these registers 16 waves each, in fp32, whose chunks have half the elements, 24), each taking rows in turn: with a quarter
+// more, the rest runs by itself at the end (16384 x 4096 bf16: 1024 workgroups 110 us, 1280 145).  At least four turns each if that still makes 256: each writes a row of shares of dw (2048 x 2048
+// fp32: 512 workgroups 19.5 us, 1536 22.4).  Up to four turns of rows are left to one workgroup, which then writes dw itself (16 rows of 512: one launch instead of two, and no workspace).
+int bwd_wgs(int64_t rows, int chunks, int dtype) {
   const int rpb = chunks <= 128 ? 4 : 1;
-  const int64_t need = (rows + rpb - 1) / rpb;
-  return (int)(need <= 4 ? 1 : need < 1024 ? need : 1024);
+  const int waves = chunks <= 256 && chunks > 128 ? 2 : chunks <= 768 ? 4 : chunks <= 1024 ? 8 : chunks <= 1536 ? 12 : 16;      // of a workgroup
+  const int64_t most = 256 * (chunks > 512 && chunks <= 768 ? (dtype == CAGC_F32 ? 4 : 3) : (dtype == CAGC_F32 ? 24 : 16) / waves);
+  const int64_t turns = (rows + rpb - 1) / rpb, want = turns / 4 > 256 ? turns / 4 : 256;
+  if (turns <= 4) return 1;
+  const int64_t wgs = want < most ? want : most;
+  return (int)(turns < wgs ? turns : wgs);
 }
 
 template <class T, class W> int launch_bwd(const NormBwd& a, void* dw, hipStream_t st, const char* what) {
-  const int chunks = (a.dim + Row<T>::V - 1) / Row<T>::V, wgs = bwd_wgs(a.rows, chunks);
-#define CAGC_CALL(TPR, NV) hipLaunchKernelGGL((k_rms_norm_bwd<T, W, TPR, NV>), dim3(wgs), dim3(TPR < 256 ? 256 : TPR), 0, st, a)
+  const int chunks = (a.dim + Row<T>::V - 1) / Row<T>::V, wgs = bwd_wgs(a.rows, chunks, sizeof(T) == 4 ? CAGC_F32 : CAGC_BF16);
+#define CAGC_CALL(TPR, NV) hipLaunchKernelGGL((k_rms_norm_bwd<T, W, TPR, NV>), dim3(wgs), dim3(threads_of(TPR)), 0, st, a)
   CAGC_ROW_SHAPES(chunks, CAGC_CALL)
 #undef CAGC_CALL
   int rc = check_launch(what);
   if (rc != CAGC_OK || !a.part) return rc;
-  hipLaunchKernelGGL((k_rms_norm_dw<W>), dim3((a.dim + 63) / 64), dim3(1024), 0, st, static_cast<W*>(dw), a.part, wgs, a.dim);
+  hipLaunchKernelGGL((k_column_sums<W>), dim3((a.dim + 15) / 16), dim3(1024), 0, st, static_cast<W*>(dw), a.part, wgs, a.dim);
   return check_launch(what);
 }
 
@@ -345,7 +374,7 @@ extern "C" int cagc_quantize_rows_e4m3(void* q, float* scale, const void* x, int
 }
 extern "C" int64_t cagc_rms_norm_bwd_workspace(int64_t rows, int64_t dim, int dtype) {
   if (rows <= 0 || !row_type(dtype) || !dim_ok(dim, dtype)) return 0;
-  const int wgs = bwd_wgs(rows, chunks_of(dim, dtype));
+  const int wgs = bwd_wgs(rows, chunks_of(dim, dtype), dtype);
   return wgs > 1 ? 4 * dim * wgs : 0;
 }
 extern "C" int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, const void* dh, const void* h, const void* w, const float* rstd, int64_t rows,
@@ -354,7 +383,7 @@ extern "C" int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, c
   CAGC_NORM_CHECKS(what);
   CAGC_REQUIRE(rows > 0, "%s: no rows (the weight's gradient is zero)", what);
   if (!dx && !dw) return CAGC_OK;
-  const bool alone = bwd_wgs(rows, chunks_of(dim, dtype)) == 1;
+  const bool alone = bwd_wgs(rows, chunks_of(dim, dtype), dtype) == 1;
   CAGC_REQUIRE(dy && h && rstd && (!dw || alone || ws), "%s: null pointer", what);
   const NormBwd a = {dx, dw && !alone ? static_cast<float*>(ws) : nullptr, alone ? dw : nullptr, dy, dh, h, w, rstd, rows, dy_stride, dh_stride, h_stride, (int)dim};
   hipStream_t st = as_stream(stream);

@@ -41,4 +41,21 @@ template <int V, class T> __device__ __forceinline__ void store_v(T* p, const fl
   }
 }
 
+// out[c] = sum over r of part[r][c], in a fixed order: a workgroup of 1024 makes 16 columns, 64 rows at a time
+template <class T> __global__ __launch_bounds__(1024) void k_column_sums(T* __restrict__ out, const float* __restrict__ part, int rows, int cols) {
+  __shared__ float sh[64][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
+  float s = 0.f;
+  if (c < cols)
+#pragma unroll 4
+    for (int r = y; r < rows; r += 64) s += part[(int64_t)r * cols + c];
+  sh[y][x] = s;
+  __syncthreads();
+  for (int half = 32; half > 0; half /= 2) {
+    if (y < half) sh[y][x] += sh[y + half][x];
+    __syncthreads();
+  }
+  if (y == 0 && c < cols) out[c] = (T)sh[0][x];
+}
+
 }  // namespace cagc

@@ -575,14 +575,13 @@ __global__ __launch_bounds__(256) void k_pad_rows(Pad a, Pad b, int64_t blocks_a
 
 // dz [rows, ldz] from the saved pre-activations and dy (zeros behind 2n), 8 or 4 columns a thread (16 bytes of dz), and the column sums of a band of rows
 // for db.  Bound by its bytes: dy, 3 planes of 16 bits (2 of fp32) and dz's two halves.
-constexpr int BAND = 64;      // rows of a workgroup
 template <class T> __global__ __launch_bounds__(256) void k_dz(T* __restrict__ z, float* __restrict__ dbpart, const T* __restrict__ dy, int64_t lddy, const void* __restrict__ saved,
-                                                              int rows, int n, int64_t ldz, int act) {
+                                                              int rows, int n, int64_t ldz, int act, int band) {
   constexpr int V = 16 / (int)sizeof(T), GROUPS = 32;      // 32 threads side by side, 8 rows at a time
   __shared__ float join[8][GROUPS][2 * V + 1];
   const int x = threadIdx.x % GROUPS, y = threadIdx.x / GROUPS;
   const int64_t c = ((int64_t)blockIdx.x * GROUPS + x) * V, plane = (int64_t)rows * n, left = n - c;
-  const int r0 = blockIdx.y * BAND, r1 = min(rows, r0 + BAND);
+  const int r0 = blockIdx.y * band, r1 = min(rows, r0 + band);
   float sg[V], su[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sg[i] = su[i] = 0.f;
@@ -643,21 +642,33 @@ int esize(int dtype) { return dtype == CAGC_F32 ? 4 : dtype == CAGC_E4M3 ? 1 : 2
 int64_t up16(int64_t b) { return (b + 15) / 16 * 16; }
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
-struct Plan { int bp, bq, splits; };      // bp = 0: the kernel for few rows (bq rows a workgroup)
+struct Plan { int bp, bq, splits; };
 
-// Tile and K split of a product with `cols` columns (of 2 `cols` rows of p when gated), `rows` rows and K of `ksteps` times 128 bytes.
-Plan plan_of(bool gated, int64_t rows, int64_t cols, int ksteps) {
-  Plan p;
+// Tile and K split of a product with `cols` columns (of 2 `cols` rows of p when gated), `rows` rows and K of `ksteps` times 128 bytes: the least of an estimate.  A workgroup's stage of 128 bytes takes
+// its latency `least`, and n workgroups of a CU take n times `share`, whichever is longer (us, measured with 128 to 4500 rows of 256 to 4096: the estimates are within 15 % of most times); `turn` is what a
+// round of workgroups spends outside its stages.  Small tiles share operands less, so they cost more a product, but come before a split of K, whose slabs want a launch of their own to be joined: 1024 x 1024 ->
+// 1024 bf16 with tiles of 128 / 64 / 32 rows 12.0 / 9.4 / 8.8 us, of 128 in two pieces of K 19.9; 512 x 4096 -> 4096 43 / 40 / 58 us.
+struct Cost { int bp, bq, slots; double least, share, turn; };
+constexpr Cost COSTS_16[] = {{256, 256, 1, 1.05, 1.55, 8.}, {128, 128, 2, .65, .47, 3.}, {128, 64, 3, .45, .30, 2.5}, {128, 32, 4, .36, .23, 2.}};
+// fp32: bound by the matrix cores at every tile
+constexpr Cost COSTS_32[] = {{256, 256, 1, 8.2, 8.2, 8.}, {128, 128, 2, 2.1, 2.1, 3.}, {128, 64, 3, 1.1, 1.03, 2.5}, {128, 32, 4, .6, .52, 2.}};
+Plan plan_of(bool gated, int64_t rows, int64_t cols, int ksteps, int dtype) {
   const int64_t prows = gated ? 2 * cols : cols;
-  auto wgs = [&](int bp, int bq) { return ((prows + bp - 1) / bp) * ((rows + bq - 1) / bq); };
-  if (rows > 128 && wgs(256, 256) >= 192) { p = {256, 256, 1}; return p; }
-  p = {128, rows <= 32 ? 32 : rows <= 64 ? 64 : 128, 1};
-  const int64_t w = wgs(p.bp, p.bq);
-  int64_t s = w >= 256 ? 1 : (512 + w - 1) / w;
-  if (s > ksteps / 4) s = ksteps / 4;      // at least 512 bytes of K a piece
-  if (s > 16) s = 16;
-  p.splits = s < 1 ? 1 : (int)s;
-  return p;
+  Plan best = {0, 0, 1};
+  double least = 0.;
+  for (const Cost& c : dtype == CAGC_F32 ? COSTS_32 : COSTS_16) {
+    const int64_t tiles = ((prows + c.bp - 1) / c.bp) * ((rows + c.bq - 1) / c.bq);
+    for (int s = 1; s <= (c.bq == 256 ? 1 : 16); ++s) {
+      if (s > 1 && (s * 4 > ksteps || tiles * s > 1024)) break;      // at least 512 bytes of K a piece
+      const int64_t wgs = tiles * s, n = (wgs + 255) / 256;
+      // the largest tile's share falls towards its latency on a chip that is not full
+      const double share = c.bq == 256 && n == 1 && dtype != CAGC_F32 ? c.least + (c.share - c.least) * wgs / 256. : n * c.share;
+      double t = (double)((ksteps + s - 1) / s) * (share > c.least ? share : c.least) + c.turn * ((n + c.slots - 1) / c.slots);
+      if (s > 1) t += 5. + 8e-6 / 5. * s * rows * prows;
+      if (best.bp == 0 || t < least) { best = {c.bp, c.bq, s}; least = t; }
+    }
+  }
+  return best;
 }
 
 template <class T, class O, int EPI, bool DP = false, bool DQ = false> int launch_product(Product& a, const Plan& p, hipStream_t st, const char* what) {
@@ -691,7 +702,7 @@ FwdLayout fwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, i
   l.kpad = up16(kb);
   l.few = few_rows_do(rows, n, kb);
   if (l.few) return l;
-  l.plan = plan_of(true, rows, n, (int)((l.kpad + 127) / 128));
+  l.plan = plan_of(true, rows, n, (int)((l.kpad + 127) / 128), dtype);
   int64_t at = 0;
   if (!x_ok) { l.xpad = at; at += up256(rows * l.kpad); }
   if (!w_ok) { l.wpad = at; at += up256(2 * n * l.kpad); }
@@ -731,6 +742,9 @@ bool sizes_ok(int64_t rows, int64_t n, int64_t k, int dtype) {
   return rows >= 0 && n > 0 && k > 0 && rows < (1ll << 31) - 512 && n < (1 << 29) && k * esize(dtype) <= MOST_LD;
 }
 
+// rows of a workgroup of k_dz: 8, a row a thread, while that makes few workgroups; 16 (each band writes a row of shares of db)
+int band_of(int64_t rows, int64_t n) { return rows * n < (1 << 20) ? 8 : 16; }
+
 struct BwdLayout { int64_t z, wpad, xpad, dbpart, slab, total; int64_t ldz, kpad; Plan dx, dw; };
 BwdLayout bwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, int dtype, bool need_dx, bool need_dw, bool need_db) {
   BwdLayout l = {};
@@ -740,17 +754,17 @@ BwdLayout bwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, i
   int64_t at = 0, s = 0;
   if (need_dx || need_dw) at += up256(rows * l.ldz * e);
   if (need_dx) {
-    l.dx = plan_of(false, rows, k, (int)((2 * n + rk - 1) / rk));
+    l.dx = plan_of(false, rows, k, (int)((2 * n + rk - 1) / rk), dtype);
     if (!w_ok) { l.wpad = at; at += up256(2 * n * l.kpad); }
     if (l.dx.splits > 1) s = 4 * (int64_t)l.dx.splits * rows * k;
   }
   if (need_dw) {
-    l.dw = plan_of(false, 2 * n, k, (int)((rows + rk - 1) / rk));
+    l.dw = plan_of(false, 2 * n, k, (int)((rows + rk - 1) / rk), dtype);
     if (!x_ok) { l.xpad = at; at += up256(rows * l.kpad); }
     const int64_t t = l.dw.splits > 1 ? 4 * (int64_t)l.dw.splits * 2 * n * k : 0;
     if (t > s) s = t;
   }
-  if (need_db) { l.dbpart = at; at += up256(4 * ((rows + BAND - 1) / BAND) * 2 * n); }
+  if (need_db) { l.dbpart = at; const int band = band_of(rows, n); at += up256(4 * ((rows + band - 1) / band) * 2 * n); }
   l.slab = at;
   l.total = at + up256(s);
   return l;
@@ -763,8 +777,8 @@ template <class T> int backward(void* dx, void* dw, void* db, char* ws, const vo
   const BwdLayout l = bwd_layout(rows, n, k, x_ok, w_ok, dtype, dx != nullptr, dw != nullptr, db != nullptr);
   T* z = dx || dw ? (T*)(ws + l.z) : nullptr;
   float* part = db ? (float*)(ws + l.dbpart) : nullptr;
-  const int bands = cdiv(rows, BAND);
-  hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)((n + 32 * v - 1) / (32 * v)), (unsigned)bands), dim3(256), 0, st, z, part, (const T*)dy, lddy, saved, (int)rows, (int)n, l.ldz, act);
+  const int band = band_of(rows, n), bands = cdiv(rows, band);
+  hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)((n + 32 * v - 1) / (32 * v)), (unsigned)bands), dim3(256), 0, st, z, part, (const T*)dy, lddy, saved, (int)rows, (int)n, l.ldz, act, band);
   int rc = check_launch(what);
   if (rc != CAGC_OK) return rc;
   if (db) {
@@ -868,7 +882,7 @@ extern "C" int cagc_gated_linear_bwd(void* dx, void* dw, void* db, void* ws, con
   const char* what = "cagc_gated_linear_bwd";
   CAGC_REQUIRE(dtype == CAGC_F32 || dtype == CAGC_F16 || dtype == CAGC_BF16, "%s: element type %d", what, dtype);
   CAGC_REQUIRE(sizes_ok(rows, n, k, dtype) && ldx >= k && ldw >= k && lddy >= n, "%s: bad sizes", what);
-  CAGC_REQUIRE((2 * n + 16) * esize(dtype) <= MOST_LD && (rows + 16) * esize(dtype) <= MOST_LD, "%s: n or rows too large (reductions of at most %lld bytes a row)", what, (long long)MOST_LD);
+  CAGC_REQUIRE((2 * n + 16) * esize(dtype) <= MOST_LD && rows <= 8 * 65535, "%s: n or rows too large (2n values of at most %lld bytes, %d rows)", what, (long long)MOST_LD, 8 * 65535);
   CAGC_REQUIRE(act == CAGC_ACT_SILU || act == CAGC_ACT_GELU, "%s: activation %d", what, act);
   CAGC_REQUIRE(rows > 0, "%s: no rows (the gradients of weight and bias are zero)", what);
   if (!dx && !dw && !db) return CAGC_OK;

@@ -508,7 +508,9 @@ template <class T, class O, int MQ, int C> __global__ __launch_bounds__(1024) vo
       for (int i = 0; i < P; ++i) acc[j][i] = mma128<T>(x[i], z[j], acc[j][i]);
   };
   const int whole = a.kbytes / 128;
-  for (int k = w; k < whole; k += nw) {
+  // a piece of the rows each, in one stretch (every nw-th 128 bytes instead: 1 x 8192 -> 4096 bf16 33.6 instead of 29.0 us, 1 x 4096 -> 8192 fp32 56 instead of 48)
+  const int q0 = (int)((int64_t)whole * w / nw), q1 = (int)((int64_t)whole * (w + 1) / nw);
+  for (int k = q0; k < q1; ++k) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -518,7 +520,7 @@ template <class T, class O, int MQ, int C> __global__ __launch_bounds__(1024) vo
     }
     mul();
   }
-  if (whole * 128 < a.kbytes && whole % nw == w) {
+  if (whole * 128 < a.kbytes && w == nw - 1) {
     const int64_t o = whole * 128ll + c0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -723,12 +725,12 @@ int pad_rows(const Pad* jobs, int count, hipStream_t st, const char* what) {
 template <class T, class O, int MQ, int C> int launch_few(Product& a, hipStream_t st, const char* what) {
   const int blocks = cdiv(a.np, C);
   int nw = 4;                              // waves that share K: more where there are few workgroups, at least 2 turns each
-  while (nw < 16 && blocks * nw < 4096 && a.kbytes >= 512 * nw) nw *= 2;
+  while (nw < 16 && blocks * nw < 8192 && a.kbytes >= 512 * nw) nw *= 2;
   hipLaunchKernelGGL((k_few_rows<T, O, MQ, C>), dim3(blocks), dim3(nw * 64), (size_t)nw / 2 * MQ * (C / 8) * 64 * sizeof(f32x4), st, a);      // (at most 64 KB)
   return check_launch(what);
 }
 template <class T, class O> int few_rows(Product& a, hipStream_t st, const char* what) {
-  const bool narrow = a.np < 16 * 256;
+  const bool narrow = a.np < 16 * 256 || a.nq <= 4;      // few rows of x: reading them in twice the workgroups costs little (1 x 4096 -> 8192 bf16 28.6 -> 25.3 us; with 16 rows 33.6 -> 35.4)
   if (a.nq <= 16) return narrow ? launch_few<T, O, 1, 8>(a, st, what) : launch_few<T, O, 1, 16>(a, st, what);
   if (a.nq <= 32) return narrow ? launch_few<T, O, 2, 8>(a, st, what) : launch_few<T, O, 2, 16>(a, st, what);
   return narrow ? launch_few<T, O, 4, 8>(a, st, what) : launch_few<T, O, 4, 16>(a, st, what);

@@ -471,11 +471,19 @@ template <class O, int EPI> __global__ __launch_bounds__(256) void k_join(Produc
 // waves have on the way (more turns' loads at once changed nothing), so where there are fewer workgroups than CUs their number decides.
 // Rows need no alignment: the loads are 16 bytes from any address.
 __device__ __forceinline__ i32x4 load16(const char* p) { return __builtin_bit_cast(i32x4, *reinterpret_cast<const Any16*>(p)); }
-// chunk of 16 bytes at `at` of a row of kbytes: zero behind its end
+// chunk of 16 bytes at `at` of a row of kbytes: zero behind its end (the row's last 16 bytes, shifted down)
 __device__ __forceinline__ i32x4 chunk_at(const char* row, int64_t at, int64_t kbytes) {
   if (at + 16 <= kbytes) return load16(row + at);
-  union { uint8_t b[16]; i32x4 v; } u;
+  union { uint8_t b[16]; uint64_t q[2]; i32x4 v; } u;
   u.v = i32x4{0, 0, 0, 0};
+  if (at >= kbytes) return u.v;
+  if (kbytes >= 16) {
+    u.v = load16(row + kbytes - 16);
+    const int s = (int)(at + 16 - kbytes) * 8;      // 8 .. 120 bits
+    u.q[0] = s < 64 ? (u.q[0] >> s | u.q[1] << (64 - s)) : u.q[1] >> (s - 64);
+    u.q[1] = s < 64 ? u.q[1] >> s : 0;
+    return u.v;
+  }
   for (int i = 0; i < 16; ++i) if (at + i < kbytes) u.b[i] = row[at + i];
   return u.v;
 }
@@ -566,13 +574,16 @@ template <class T, class O, int MQ, int C> __global__ __launch_bounds__(1024) vo
 // ---- layout passes ----------------------------------------------------------------------------------------------------------------
 // rows of any stride and alignment -> rows of whole 16-byte chunks, the rest of the last chunk zero; up to two operands in one launch
 struct Pad { char* dst; const char* src; int64_t rows, kbytes, ld; };
-__global__ __launch_bounds__(256) void k_pad_rows(Pad a, Pad b, int64_t blocks_a) {
-  const bool second = blockIdx.x >= blocks_a;
+__global__ __launch_bounds__(256) void k_pad_rows(Pad a, Pad b) {
+  int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);      // a row a wave
+  const bool second = r >= a.rows;
   const Pad p = second ? b : a;
-  const int64_t id = (blockIdx.x - (second ? blocks_a : 0)) * 256 + threadIdx.x, width = (p.kbytes + 15) / 16;
-  if (id >= p.rows * width) return;
-  const int64_t r = id / width, c = (id - r * width) * 16;
-  *reinterpret_cast<i32x4*>(p.dst + (r * width * 16 + c)) = chunk_at(p.src + r * p.ld, c, p.kbytes);
+  if (second) r -= a.rows;
+  if (r >= p.rows) return;
+  const int64_t width = (p.kbytes + 15) / 16 * 16;
+  const char* src = p.src + r * p.ld;
+  char* dst = p.dst + r * width;
+  for (int64_t c = (threadIdx.x & 63) * 16; c < width; c += 1024) *reinterpret_cast<i32x4*>(dst + c) = chunk_at(src, c, p.kbytes);
 }
 
 // dz [rows, ldz] from the saved pre-activations and dy (zeros behind 2n), 8 or 4 columns a thread (16 bytes of dz), and the column sums of a band of rows
@@ -716,9 +727,9 @@ FwdLayout fwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, i
 
 int pad_rows(const Pad* jobs, int count, hipStream_t st, const char* what) {
   if (count == 0) return CAGC_OK;
-  auto blocks = [](const Pad& p) { return (p.rows * ((p.kbytes + 15) / 16) + 255) / 256; };
-  const int64_t first = blocks(jobs[0]), both = first + (count > 1 ? blocks(jobs[1]) : 0);
-  hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)both), dim3(256), 0, st, jobs[0], jobs[count - 1], first);
+  const Pad none = {};
+  const Pad& second = count > 1 ? jobs[1] : none;
+  hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)((jobs[0].rows + second.rows + 3) / 4)), dim3(256), 0, st, jobs[0], second);
   return check_launch(what);
 }
 

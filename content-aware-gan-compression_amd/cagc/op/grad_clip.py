@@ -41,6 +41,9 @@ def _launch(tensors, code, max_norm, scale, dev):
     """the norm (0-dim fp32); with `scale`, the tensors are clipped in place"""
     flat, n = tensors, len(tensors)
     if not all(map(_T.is_contiguous, tensors)):
+        starts = [t.data_ptr() for t in tensors if t.numel()]
+        if len(set(starts)) < len(starts):      # (the library sees their copies)
+            raise RuntimeError("cagc_clip_grad_norm: two tensors of the list share memory")
         flat = [t.contiguous() for t in tensors]
     p, sizes = array("Q", map(_T.data_ptr, flat)), array("q", map(_T.numel, flat))
     types = array("i", map(_CODES.__getitem__, map(_dtype, flat)))

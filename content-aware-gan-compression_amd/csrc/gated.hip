@@ -11,8 +11,6 @@ namespace cagc {
 namespace gated {
 namespace {
 
-enum { EPI_GATED = 0, EPI_PLAIN = 1 };
-
 struct Product {
   const char* p;         // operand of the output's columns (gated: gate rows, then up rows from p2)
   const char* p2;
@@ -100,7 +98,7 @@ template <class T, int BQ, bool DP> struct Stages {
   static constexpr int SB = FIVE ? 64 : 128, NS = FIVE ? 5 : 2;
 };
 
-template <class T, class O, int BP, int BQ, int WP, int WQ, int EPI, bool DP, bool DQ> struct Tile {      // (O: a class of its own for each kernel)
+template <class T, class O, int BP, int BQ, int WP, int WQ, bool DP, bool DQ> struct Tile {      // (O: a class of its own for each kernel)
   static constexpr int SB = Stages<T, BQ, DP>::SB, NS = Stages<T, BQ, DP>::NS;
   typedef Side<T, BP, DP, SB> P;
   typedef Side<T, BQ, DQ, SB> Q;
@@ -243,10 +241,11 @@ template <class E> __device__ __forceinline__ void put4(E* p, f32x4 v, int left)
   for (int r = 0; r < 4; ++r) if (r < left) p[r] = (E)v[r];
 }
 
-template <class T, class O, int BP, int BQ, int WP, int WQ, int EPI, bool DP, bool DQ>
+// The forward has K along the rows of both and the gated epilogue; the backward's products have it down p's columns (DP), and down q's for dW (DQ).
+template <class T, class O, int BP, int BQ, int WP, int WQ, bool DP, bool DQ>
 __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
-  typedef Tile<T, O, BP, BQ, WP, WQ, EPI, DP, DQ> K;
-  constexpr bool GATED = EPI == EPI_GATED;
+  typedef Tile<T, O, BP, BQ, WP, WQ, DP, DQ> K;
+  constexpr bool GATED = !DP;
   constexpr int COLS = GATED ? BP / 2 : BP, NT = WP * WQ * 64;
   __shared__ __attribute__((aligned(1024))) char stage[K::LDS];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = w % WP, wq = w / WP;
@@ -259,9 +258,8 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
   K t;
   // first elements of the tile's operands at stage k0, and how far a stage moves them
   const int64_t dp = DP ? K::P::RK * a.ldp : K::SB, dq = DQ ? K::Q::RK * a.ldq : K::SB;
-  const int second = min(n0 + BP / 2, a.np - 1);      // (not gated, K along rows: the tile's other half of rows)
   const char* p = a.p + (DP ? (int64_t)n0 * K::P::ES : (int64_t)n0 * a.ldp) + k0 * dp;
-  const char* p2 = (GATED ? a.p2 + (int64_t)n0 * a.ldp : a.p + (int64_t)second * a.ldp) + k0 * dp;
+  const char* p2 = GATED ? a.p2 + (int64_t)n0 * a.ldp + k0 * dp : nullptr;
   const char* q = a.q + (DQ ? (int64_t)m0 * K::Q::ES : (int64_t)m0 * a.ldq) + k0 * dq;
   const int mine = w * 1024 + lane * 16;
   t.pk = K::P::first(mine);
@@ -269,8 +267,8 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
 #pragma unroll
   for (int c = 0; c < K::LP; ++c) {
     const int at = c * K::NW * 1024 + mine;
-    const bool upper = !DP && c * K::NW * 1024 >= BP / 2 * K::SB;
-    t.po[c] = K::P::source(upper ? at - BP / 2 * K::SB : at, a.ldp, a.np - 1 - (upper && !GATED ? second : n0), (a.np - n0) * K::P::ES);
+    const bool up = GATED && c * K::NW * 1024 >= BP / 2 * K::SB;
+    t.po[c] = K::P::source(up ? at - BP / 2 * K::SB : at, a.ldp, a.np - 1 - n0, (a.np - n0) * K::P::ES);
   }
 #pragma unroll
   for (int c = 0; c < K::LQ; ++c) t.qo[c] = K::Q::source(c * K::NW * 1024 + mine, a.ldq, a.nq - 1 - m0, (a.nq - m0) * K::Q::ES);
@@ -445,23 +443,23 @@ template <class O> __device__ __forceinline__ void gated_out(const Product& a, i
 }
 
 // the pieces of a K split, added in order, and the epilogue: four outputs a thread
-template <class O, int EPI> __global__ __launch_bounds__(256) void k_join(Product a) {
+template <class O, bool GATED> __global__ __launch_bounds__(256) void k_join(Product a) {
   const int quads = (a.np + 3) / 4;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= (int64_t)quads * a.nq) return;
   const int m = (int)(id / quads), n = (int)(id % quads) * 4, left = a.np - n;
-  const int64_t width = EPI == EPI_GATED ? 2 * (int64_t)a.np : a.np;
+  const int64_t width = GATED ? 2 * (int64_t)a.np : a.np;
   f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
   for (int s = 0; s < a.splits; ++s) {
     const float* p = a.slab + ((int64_t)s * a.nq + m) * width + n;
 #pragma unroll
-    for (int h = 0; h < (EPI == EPI_GATED ? 2 : 1); ++h) {
+    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
       if ((a.np & 3) == 0) v[h] += *reinterpret_cast<const f32x4*>(p + h * (int64_t)a.np);
       else
         for (int r = 0; r < 4; ++r) if (r < left) v[h][r] += p[h * (int64_t)a.np + r];
     }
   }
-  if (EPI == EPI_GATED) gated_out<O>(a, m, n, v[0], v[1]);
+  if (GATED) gated_out<O>(a, m, n, v[0], v[1]);
   else put4(static_cast<O*>(a.out) + (int64_t)m * a.ldo + n, v[0] * a.alpha, left);
 }
 
@@ -575,15 +573,13 @@ template <class T, class O, int MQ, int C> __global__ __launch_bounds__(1024) vo
 // rows of any stride and alignment -> rows of whole 16-byte chunks, the rest of the last chunk zero; up to two operands in one launch
 struct Pad { char* dst; const char* src; int64_t rows, kbytes, ld; };
 __global__ __launch_bounds__(256) void k_pad_rows(Pad a, Pad b) {
-  int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);      // a row a wave
-  const bool second = r >= a.rows;
-  const Pad p = second ? b : a;
-  if (second) r -= a.rows;
-  if (r >= p.rows) return;
-  const int64_t width = (p.kbytes + 15) / 16 * 16;
-  const char* src = p.src + r * p.ld;
-  char* dst = p.dst + r * width;
-  for (int64_t c = (threadIdx.x & 63) * 16; c < width; c += 1024) *reinterpret_cast<i32x4*>(dst + c) = chunk_at(src, c, p.kbytes);
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.rows + b.rows; i += (int64_t)gridDim.x * 4) {      // a row a wave
+    const Pad p = i < a.rows ? a : b;
+    const int64_t r = i < a.rows ? i : i - a.rows, width = (p.kbytes + 15) / 16 * 16;
+    const char* src = p.src + r * p.ld;
+    char* dst = p.dst + r * width;
+    for (int64_t c = (threadIdx.x & 63) * 16; c < width; c += 1024) *reinterpret_cast<i32x4*>(dst + c) = chunk_at(src, c, p.kbytes);
+  }
 }
 
 // dz [rows, ldz] from the saved pre-activations and dy (zeros behind 2n), 8 or 4 columns a thread (16 bytes of dz), and the column sums of a band of rows
@@ -684,20 +680,20 @@ Plan plan_of(bool gated, int64_t rows, int64_t cols, int ksteps, int dtype) {
   return best;
 }
 
-template <class T, class O, int EPI, bool DP = false, bool DQ = false> int launch_product(Product& a, const Plan& p, hipStream_t st, const char* what) {
-  const int cols = EPI == EPI_GATED ? p.bp / 2 : p.bp;
+template <class T, class O, bool DP, bool DQ> int launch_product(Product& a, const Plan& p, hipStream_t st, const char* what) {
+  const int cols = DP ? p.bp : p.bp / 2;
   a.tiles_p = cdiv(a.np, cols);
   a.tiles_q = cdiv(a.nq, p.bq);
   a.splits = p.splits;
   const dim3 grid((unsigned)(a.tiles_p * a.tiles_q), (unsigned)a.splits);
-  if (p.bp == 256) hipLaunchKernelGGL((k_product<T, O, 256, 256, 4, 2, EPI, DP, DQ>), grid, dim3(512), 0, st, a);
-  else if (p.bq == 128) hipLaunchKernelGGL((k_product<T, O, 128, 128, 2, 2, EPI, DP, DQ>), grid, dim3(256), 0, st, a);
-  else if (p.bq == 64) hipLaunchKernelGGL((k_product<T, O, 128, 64, 4, 1, EPI, DP, DQ>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_product<T, O, 128, 32, 4, 1, EPI, DP, DQ>), grid, dim3(256), 0, st, a);
+  if (p.bp == 256) hipLaunchKernelGGL((k_product<T, O, 256, 256, 4, 2, DP, DQ>), grid, dim3(512), 0, st, a);
+  else if (p.bq == 128) hipLaunchKernelGGL((k_product<T, O, 128, 128, 2, 2, DP, DQ>), grid, dim3(256), 0, st, a);
+  else if (p.bq == 64) hipLaunchKernelGGL((k_product<T, O, 128, 64, 4, 1, DP, DQ>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_product<T, O, 128, 32, 4, 1, DP, DQ>), grid, dim3(256), 0, st, a);
   int rc = check_launch(what);
   if (rc != CAGC_OK || a.splits == 1) return rc;
   const int64_t quads = (int64_t)((a.np + 3) / 4) * a.nq;
-  hipLaunchKernelGGL((k_join<O, EPI>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_join<O, !DP>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, a);
   return check_launch(what);
 }
 // 16-byte alignment of a matrix's rows and row length: what the tiled product's loads want
@@ -729,7 +725,8 @@ int pad_rows(const Pad* jobs, int count, hipStream_t st, const char* what) {
   if (count == 0) return CAGC_OK;
   const Pad none = {};
   const Pad& second = count > 1 ? jobs[1] : none;
-  hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)((jobs[0].rows + second.rows + 3) / 4)), dim3(256), 0, st, jobs[0], second);
+  const int64_t wgs = (jobs[0].rows + second.rows + 3) / 4, most = 1 << 20;
+  hipLaunchKernelGGL(k_pad_rows, dim3((unsigned)(wgs < most ? wgs : most)), dim3(256), 0, st, jobs[0], second);
   return check_launch(what);
 }
 
@@ -748,7 +745,7 @@ template <class T, class O> int few_rows(Product& a, hipStream_t st, const char*
 }
 
 template <class T, class O> int forward(Product& a, const FwdLayout& l, hipStream_t st, const char* what) {
-  return l.few ? few_rows<T, O>(a, st, what) : launch_product<T, O, EPI_GATED>(a, l.plan, st, what);
+  return l.few ? few_rows<T, O>(a, st, what) : launch_product<T, O, false, false>(a, l.plan, st, what);
 }
 
 bool sizes_ok(int64_t rows, int64_t n, int64_t k, int dtype) {
@@ -814,14 +811,14 @@ template <class T> int backward(void* dx, void* dw, void* db, char* ws, const vo
     a.nq = (int)rows;
     a.kbytes = (int)(l.ldz * e); a.krows = (int)(2 * n);
     a.out = dx;
-    if ((rc = launch_product<T, T, EPI_PLAIN, true, false>(a, l.dx, st, what)) != CAGC_OK) return rc;
+    if ((rc = launch_product<T, T, true, false>(a, l.dx, st, what)) != CAGC_OK) return rc;
   }
   if (dw) {                                  // dz and x [rows, k] down their columns
     a.p = x_ok ? (const char*)x : ws + l.xpad; a.ldp = x_ok ? ldx * e : l.kpad;
     a.nq = (int)(2 * n);
     a.kbytes = 0; a.krows = (int)rows;
     a.out = dw;
-    if ((rc = launch_product<T, T, EPI_PLAIN, true, true>(a, l.dw, st, what)) != CAGC_OK) return rc;
+    if ((rc = launch_product<T, T, true, true>(a, l.dw, st, what)) != CAGC_OK) return rc;
   }
   return CAGC_OK;
 }

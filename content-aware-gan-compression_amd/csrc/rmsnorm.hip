@@ -298,12 +298,28 @@ bool row_type(int dtype) { return dtype == CAGC_F32 || dtype == CAGC_F16 || dtyp
 int chunks_of(int64_t dim, int dtype) { return (int)((dim * esize(dtype) + 15) / 16); }
 bool dim_ok(int64_t dim, int dtype) { return dim > 0 && dim * esize(dtype) <= (int64_t)MOST_CHUNKS * 16; }
 
-template <class T, class W, int OUT> int launch_norm(const Norm& a, hipStream_t st, const char* what) {
+template <class T, class W, int OUT> int launch_some(const Norm& a, hipStream_t st, const char* what) {
   const int chunks = (a.dim + Row<T>::V - 1) / Row<T>::V;
 #define CAGC_CALL(TPR, NV) hipLaunchKernelGGL((k_rms_norm<T, W, TPR, NV, OUT>), dim3((unsigned)((a.rows + threads_of(TPR) / TPR - 1) / (threads_of(TPR) / TPR))), dim3(threads_of(TPR)), 0, st, a)
   CAGC_ROW_SHAPES(chunks, CAGC_CALL)
 #undef CAGC_CALL
   return check_launch(what);
+}
+// a launch holds fewer than 2^32 threads: at most 2^21 rows at a time
+template <class T, class W, int OUT> int launch_norm(Norm a, hipStream_t st, const char* what) {
+  const int64_t rows = a.rows, most = 1 << 21, out = OUT == 0 ? (int64_t)sizeof(T) : 1;
+  for (int64_t done = 0; done < rows; done += most) {
+    a.rows = rows - done < most ? rows - done : most;
+    const int rc = launch_some<T, W, OUT>(a, st, what);
+    if (rc != CAGC_OK) return rc;
+    a.y = static_cast<char*>(a.y) + most * a.dim * out;
+    a.x = static_cast<const T*>(a.x) + most * a.xs;
+    if (a.res) a.res = static_cast<const T*>(a.res) + most * a.rs;
+    if (a.h) a.h = static_cast<T*>(a.h) + most * a.dim;
+    if (a.rstd) a.rstd += most;
+    if (a.scale) a.scale += most;
+  }
+  return CAGC_OK;
 }
 template <int OUT> int launch_norm_as(const Norm& a, int dtype, int wdtype, hipStream_t st, const char* what) {
   if (dtype == CAGC_F32) return launch_norm<float, float, OUT>(a, st, what);

@@ -113,25 +113,26 @@ def test_forward_and_gradients(case, dev):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dt", [F32, BF16], ids=str)
-def test_large_tiles(dt):
-    """sizes that the 256 x 256 tiles take in every product, checked on a sample of rows and columns"""
-    rows, k, n = 4100, 1024, 2056
-    x, w = make((rows, k), dt, "cuda", 1).requires_grad_(True), make((2 * n, k), dt, "cuda", 2).requires_grad_(True)
+@pytest.mark.parametrize("dt", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("rows, k, n, act", [(2040, 2048, 4090, "gelu"), (4100, 4090, 1030, "silu"), (1250, 700, 4400, "gelu"), (3000, 256, 900, "silu")])
+def test_large_tiles(rows, k, n, act, dt):
+    """sizes that the larger tiles take, with and without a split of K, in every product"""
+    scale = 1 / math.sqrt(k)
+    x, w, b = make((rows, k), dt, "cuda", 1).requires_grad_(True), make((2 * n, k), dt, "cuda", 2).requires_grad_(True), make((2 * n,), dt, "cuda", 4, 0.3).requires_grad_(True)
     dy = make((rows, n), dt, "cuda", 3)
-    y = gated_linear(x, w, scale=1 / 32)
-    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    y = gated_linear(x, w, b, activation=act, scale=scale)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
     xd, wd = x.detach().double(), w.detach().double()
-    z = xd @ wd.t().contiguous() / 32
-    a, da = act64("silu", z[:, :n])
+    z = xd @ wd.t().contiguous() * scale + b.detach().double()
+    a, da = act64(act, z[:, :n])
     u = z[:, n:]
     dz = torch.cat([dy.double() * u * da, dy.double() * a], 1)
-    # |z| <= 6, so a term's tolerance is taken as a whole from its largest: 3 u_T of values of this size, and random signs over the sums
+    # two roundings to the type (dz, the result), each below u_T in the mean, and the fp32 sums: 2^-24 sqrt(terms) in the mean, 2^-24 * 64 at these sizes
     ut = unit(dt) + 64 * E
-    for got, want, terms in ((y, a * u, 1), (dx, dz @ wd / 32, 2 * n), (dw, dz.t().contiguous() @ xd / 32, rows)):
+    for what, got, want in (("y", y, a * u), ("dx", dx, dz @ wd * scale), ("dw", dw, dz.t().contiguous() @ xd * scale), ("db", db, dz.sum(0))):
         err = (got.detach().double() - want)
-        assert float(err.norm() / want.norm()) < 2 * ut      # two roundings (dz, result), each below u_T in the mean
-        assert float(err.abs().max()) < 16 * ut * float(want.abs().max())
+        assert float(err.norm() / want.norm()) < 2 * ut, what
+        assert float(err.abs().max()) < 16 * ut * float(want.abs().max()), what
 
 
 @pytest.mark.gpu
@@ -155,7 +156,7 @@ def test_gradient_against_differences():
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("case", [(1, 64, 64, BF16, False), (16, 1024, 100, BF16, True), (5, 33, 7, F16, True), (31, 200, 48, F32, False), (50, 129, 65, BF16, True),
-                                  (200, 512, 300, BF16, False), (1000, 640, 1030, F32, True)], ids=str)
+                                  (200, 512, 300, BF16, False), (1000, 640, 1030, F32, True), (1500, 2100, 1100, BF16, True)], ids=str)
 def test_e4m3(case, dev):
     rows, k, n, dt, bias = case
     xq, xs = quantize_rows_e4m3(make((rows, k), F32, dev, 1))

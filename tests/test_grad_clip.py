@@ -123,7 +123,8 @@ def test_refusals(dev):
 @pytest.mark.gpu
 def test_refusals_of_the_kernels():
     g = torch.randn(64, device="cuda")
-    for bad in ([g, g], [g[:40], g[30:]], [g, torch.randn(3)], [g.double()], [g.to(torch.float8_e4m3fn)], [g, g[5:6]]):
+    part = torch.randn(8, 8, device="cuda")[:, 2:5]
+    for bad in ([part, part], [g, g], [g[:40], g[30:]], [g, torch.randn(3)], [g.double()], [g.to(torch.float8_e4m3fn)], [g, g[5:6]]):
         with pytest.raises(RuntimeError):
             get_total_norm(bad)
         with pytest.raises(RuntimeError):

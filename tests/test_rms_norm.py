@@ -172,6 +172,21 @@ def test_no_rows_and_the_sum_alone(dev):
     assert torch.equal(gx, torch.ones_like(gx))
 
 
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_holds():
+    rows = (1 << 21) * 2 + 5
+    x = torch.randn(rows, 3, device="cuda", dtype=BF16)
+    r = torch.randn(rows, 3, device="cuda", dtype=BF16)
+    y, h = rms_norm(x, residual=r)
+    q, s, h2 = rms_norm_e4m3(x, residual=r)
+    assert torch.equal(h, x + r) and torch.equal(h2, h)
+    for at in (0, (1 << 21) - 2, (1 << 21) + 1, rows - 4):
+        part = slice(at, at + 4)
+        one, _ = rms_norm(x[part], residual=r[part])
+        q1, s1, _ = rms_norm_e4m3(x[part], residual=r[part])
+        assert torch.equal(y[part], one) and torch.equal(q[part].float(), q1.float()) and torch.equal(s[part], s1)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_refusals(dev):
     x, w = torch.randn(3, 8, device=dev), torch.ones(8, device=dev)

@@ -732,8 +732,9 @@ int pad_rows(const Pad* jobs, int count, hipStream_t st, const char* what) {
 
 template <class T, class O, int MQ, int C> int launch_few(Product& a, hipStream_t st, const char* what) {
   const int blocks = cdiv(a.np, C);
-  int nw = 4;                              // waves that share K: more where there are few workgroups, at least 2 turns each
-  while (nw < 16 && blocks * nw < 8192 && a.kbytes >= 512 * nw) nw *= 2;
+  // waves that share K: more where there are few workgroups, at least 2 turns each (16 columns: 16 x 4096 -> 8192 e4m3 with 8 waves 13.9 us, with 16 15.6; 8 columns: 1 x 4096 -> 8192 bf16 26.4 and 25.6)
+  int nw = 4;
+  while (nw < 16 && blocks * nw < (C == 8 ? 8192 : 4096) && a.kbytes >= 512 * nw) nw *= 2;
   hipLaunchKernelGGL((k_few_rows<T, O, MQ, C>), dim3(blocks), dim3(nw * 64), (size_t)nw / 2 * MQ * (C / 8) * 64 * sizeof(f32x4), st, a);      // (at most 64 KB)
   return check_launch(what);
 }

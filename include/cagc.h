@@ -13,7 +13,8 @@
  * Conventions
  *   - plain C, no torch / ATen types: raw device pointers, sizes, a hipStream_t passed as void*.
  *   - all tensors are fp32, contiguous, NCHW unless stated ("planes" = N*C flattened); the two reference operators also
- *     exist in an any-dtype form (fp32 / fp16 / fp64: cagc_fused_bias_act_any, cagc_upfirdn2d_any).
+ *     exist in an any-dtype form (fp32 / fp16 / fp64: cagc_fused_bias_act_any, cagc_upfirdn2d_any), and the row-wise, gated
+ *     and gradient-norm operators at the end of this file take element types, row strides and any alignment.
  *   - OWNERSHIP: the caller allocates every output and workspace (PyTorch caching allocator) and passes data_ptr();
  *     the library never frees or retains a caller's pointer.  TWO exceptions to "never allocates", both library-owned
  *     scratches kept per (device, stream), obtained with hipMalloc on first use (also under stream capture, relaxed

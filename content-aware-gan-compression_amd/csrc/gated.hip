@@ -590,7 +590,7 @@ template <class T> __global__ __launch_bounds__(256) void k_dz(T* __restrict__ z
   __shared__ float join[8][GROUPS][2 * V + 1];
   const int x = threadIdx.x % GROUPS, y = threadIdx.x / GROUPS;
   const int64_t c = ((int64_t)blockIdx.x * GROUPS + x) * V, plane = (int64_t)rows * n, left = n - c;
-  const int r0 = blockIdx.y * band, r1 = min(rows, r0 + band);
+  const int r0 = blockIdx.y * band, r1 = r0 + min(band, rows - r0);
   float sg[V], su[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sg[i] = su[i] = 0.f;
@@ -750,11 +750,15 @@ template <class T, class O> int forward(Product& a, const FwdLayout& l, hipStrea
 }
 
 bool sizes_ok(int64_t rows, int64_t n, int64_t k, int dtype) {
-  return rows >= 0 && n > 0 && k > 0 && rows < (1ll << 31) - 512 && n < (1 << 29) && k * esize(dtype) <= MOST_LD;
+  return rows >= 0 && n > 0 && k > 0 && rows < (1ll << 31) - 512 && n <= (1 << 26) && k * esize(dtype) <= MOST_LD;
 }
 
-// rows of a workgroup of k_dz: 8, a row a thread, while that makes few workgroups; 16 (each band writes a row of shares of db)
-int band_of(int64_t rows, int64_t n) { return rows * n < (1 << 20) ? 8 : 16; }
+// rows of a workgroup of k_dz: 8, a row a thread, while that makes few workgroups; 16 (each band writes a row of shares of db); as many more as keep the grid to 65535 of them
+int band_of(int64_t rows, int64_t n) {
+  int64_t band = rows * n < (1 << 20) ? 8 : 16;
+  while (rows > band * 65535) band *= 2;
+  return (int)band;
+}
 
 struct BwdLayout { int64_t z, wpad, xpad, dbpart, slab, total; int64_t ldz, kpad; Plan dx, dw; };
 BwdLayout bwd_layout(int64_t rows, int64_t n, int64_t k, bool x_ok, bool w_ok, int dtype, bool need_dx, bool need_dw, bool need_db) {
@@ -893,7 +897,7 @@ extern "C" int cagc_gated_linear_bwd(void* dx, void* dw, void* db, void* ws, con
   const char* what = "cagc_gated_linear_bwd";
   CAGC_REQUIRE(dtype == CAGC_F32 || dtype == CAGC_F16 || dtype == CAGC_BF16, "%s: element type %d", what, dtype);
   CAGC_REQUIRE(sizes_ok(rows, n, k, dtype) && ldx >= k && ldw >= k && lddy >= n, "%s: bad sizes", what);
-  CAGC_REQUIRE((2 * n + 16) * esize(dtype) <= MOST_LD && rows <= 8 * 65535, "%s: n or rows too large (2n values of at most %lld bytes, %d rows)", what, (long long)MOST_LD, 8 * 65535);
+  CAGC_REQUIRE((2 * n + 16) * esize(dtype) <= MOST_LD, "%s: n too large (2n values of at most %lld bytes)", what, (long long)MOST_LD);
   CAGC_REQUIRE(act == CAGC_ACT_SILU || act == CAGC_ACT_GELU, "%s: activation %d", what, act);
   CAGC_REQUIRE(rows > 0, "%s: no rows (the gradients of weight and bias are zero)", what);
   if (!dx && !dw && !db) return CAGC_OK;

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import cagc.model as M
+from cagc import _lib
 from cagc.op import clip_grad_norm_, gated_linear, gated_linear_e4m3, quantize_rows_e4m3, rms_norm, rms_norm_e4m3
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -220,6 +221,26 @@ def test_refusals(dev):
                 lambda: gated_linear_e4m3(q, s, wq, ws, b, out_dtype=BF16), lambda: gated_linear_e4m3(q, s, wq, ws, out_dtype=torch.float64)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", (F32, BF16), ids=str)
+def test_gradients_of_more_rows_than_bands_of_sixteen(dt):
+    """a grid holds 65535 bands of rows: 1 048 560 rows of bands of 16"""
+    rows, k, n = 1100003, 5, 3
+    x, w, b = (make(s, dt, "cuda", i).requires_grad_(True) for i, s in enumerate(((rows, k), (2 * n, k), (2 * n,)), 1))
+    dy = make((rows, n), dt, "cuda", 4)
+    grads = torch.autograd.grad(gated_linear(x, w, b, scale=0.4), (x, w, b), dy)
+    ref = reference(x, w, b, "silu", 0.4, dt, dy)
+    for g, name in zip(grads, ("dx", "dw", "db")):
+        within(g, ref[name], ref[name + "_tol"], name)
+
+
+def test_columns_beyond_a_launch_are_refused():
+    """by the sizes alone: no operands are there"""
+    lib = _lib.load()
+    assert lib.cagc_gated_linear_fwd(None, None, None, None, None, None, None, None, 1, (1 << 26) + 1, 8, 8, 8, 3, 3, 0, 1.0, None) != 0
+    assert b"bad sizes" in lib.cagc_last_error()
 
 
 @pytest.mark.gpu

@@ -449,16 +449,30 @@ template <class O, bool GATED> __global__ __launch_bounds__(256) void k_join(Pro
   if (id >= (int64_t)quads * a.nq) return;
   const int m = (int)(id / quads), n = (int)(id % quads) * 4, left = a.np - n;
   const int64_t width = GATED ? 2 * (int64_t)a.np : a.np;
+  constexpr int HALVES = GATED ? 2 : 1, AHEAD = 8;
+  const int64_t slab = a.nq * width;
+  const float* p = a.slab + m * width + n;
   f32x4 v[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-  for (int s = 0; s < a.splits; ++s) {
-    const float* p = a.slab + ((int64_t)s * a.nq + m) * width + n;
+  int s = 0;
+  if (left >= 4) {
+    for (; s + AHEAD <= a.splits; s += AHEAD, p += AHEAD * slab) {      // (16 slabs of 256 x 128: one after the other 7.1 us, 4.7; 64: 19, 6.8)
+      f32x4 e[AHEAD][HALVES];
 #pragma unroll
-    for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-      if ((a.np & 3) == 0) v[h] += *reinterpret_cast<const f32x4*>(p + h * (int64_t)a.np);
-      else
-        for (int r = 0; r < 4; ++r) if (r < left) v[h][r] += p[h * (int64_t)a.np + r];
+      for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) e[i][h] = __builtin_bit_cast(f32x4, *reinterpret_cast<const Any16*>(p + i * slab + h * (int64_t)a.np));
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) v[h] += e[i][h];
     }
   }
+  for (; s < a.splits; ++s, p += slab)
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h)
+      if (left >= 4) v[h] += __builtin_bit_cast(f32x4, *reinterpret_cast<const Any16*>(p + h * (int64_t)a.np));
+      else
+        for (int r = 0; r < 4; ++r) if (r < left) v[h][r] += p[h * (int64_t)a.np + r];
   if (GATED) gated_out<O>(a, m, n, v[0], v[1]);
   else put4(static_cast<O*>(a.out) + (int64_t)m * a.ldo + n, v[0] * a.alpha, left);
 }
@@ -657,6 +671,8 @@ struct Plan { int bp, bq, splits; };
 // its latency `least`, and n workgroups of a CU take n times `share`, whichever is longer (us, measured with 128 to 4500 rows of 256 to 4096: the estimates are within 15 % of most times); `turn` is what a
 // round of workgroups spends outside its stages.  Small tiles share operands less, so they cost more a product, but come before a split of K, whose slabs want a launch of their own to be joined: 1024 x 1024 ->
 // 1024 bf16 with tiles of 128 / 64 / 32 rows 12.0 / 9.4 / 8.8 us, of 128 in two pieces of K 19.9; 512 x 4096 -> 4096 43 / 40 / 58 us.
+// Up to 64 pieces: with 16, dW of many rows and few columns leaves CUs idle (131072 x 64 -> 128 bf16 103 instead of 79 us with dz, 65536 x 128 -> 128 fp32 106 instead of 82); 128 help one and cost another (67; 65536 x
+// 64 -> 64 41 instead of 37).
 struct Cost { int bp, bq, slots; double least, share, turn; };
 constexpr Cost COSTS_16[] = {{256, 256, 1, 1.05, 1.55, 8.}, {128, 128, 2, .65, .47, 3.}, {128, 64, 3, .45, .30, 2.5}, {128, 32, 4, .36, .23, 2.}};
 // fp32: bound by the matrix cores at every tile
@@ -667,7 +683,7 @@ Plan plan_of(bool gated, int64_t rows, int64_t cols, int ksteps, int dtype) {
   double least = 0.;
   for (const Cost& c : dtype == CAGC_F32 ? COSTS_32 : COSTS_16) {
     const int64_t tiles = ((prows + c.bp - 1) / c.bp) * ((rows + c.bq - 1) / c.bq);
-    for (int s = 1; s <= (c.bq == 256 ? 1 : 16); ++s) {
+    for (int s = 1; s <= (c.bq == 256 ? 1 : 64); ++s) {
       if (s > 1 && (s * 4 > ksteps || tiles * s > 1024)) break;      // at least 512 bytes of K a piece
       const int64_t wgs = tiles * s, n = (wgs + 255) / 256;
       // the largest tile's share falls towards its latency on a chip that is not full

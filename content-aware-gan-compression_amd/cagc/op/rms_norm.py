@@ -133,8 +133,8 @@ def rms_norm(input, weight=None, residual=None, eps=1e-6):
 def _quantize(y):
     """rows of the composed path -> (e4m3, scale)"""
     y = y.float()
-    scale = (y.abs().amax(-1) * (1 / E4M3_MAX)).clamp_min(2.0 ** -126)
-    return (y * (1 / scale)[..., None]).to(torch.float8_e4m3fn), scale
+    scale = (y.abs().amax(-1) / E4M3_MAX).clamp_min(2.0 ** -126)
+    return (y / scale[..., None]).to(torch.float8_e4m3fn), scale
 
 
 def rms_norm_e4m3(input, weight=None, residual=None, eps=1e-6):

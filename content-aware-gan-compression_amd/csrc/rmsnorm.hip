@@ -12,13 +12,26 @@ namespace {
 
 template <class T> struct Row { static constexpr int V = 16 / (int)sizeof(T); };
 
-// V e4m3 bytes
-template <int V> __device__ __forceinline__ void store_q(uint8_t* p, const float (&f)[V], float inv, int n) {
+// V e4m3 bytes of f / scale, `inv` = 1 / scale.  The quotient is the correctly rounded one: times the rounded reciprocal alone, values beside a tie of e4m3 would go to the other side.  Two residuals
+// make it so (Markstein 1990: the first leaves it within a step, the second rounds it as the division does); a scale below 2^-90, whose residuals underflow, an infinite one and a NaN are divided by.
+// 8191 x 5120 bf16: 57.8 us times the reciprocal, 62.1 divided, 58.8 this way.
+template <int V> __device__ __forceinline__ void store_q(uint8_t* p, const float (&f)[V], float scale, float inv, int n) {
+  float q[V];
+  if (scale > 0x1p-90f && scale < __builtin_inff()) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float a = f[i] * inv, b = fmaf(fmaf(-a, scale, f[i]), inv, a);
+      q[i] = fmaf(fmaf(-b, scale, f[i]), inv, b);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[i] = f[i] / scale;
+  }
   uint32_t d[V / 4];
 #pragma unroll
   for (int i = 0; i < V / 4; ++i) {
-    int v = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inv, f[4 * i + 1] * inv, 0, false);
-    d[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, v, true);
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
+    d[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], v, true);
   }
   struct __attribute__((packed, aligned(1))) Any { uint32_t v[V / 4]; };
   if (n >= V) {
@@ -136,7 +149,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_norm(Norm a) {
         float f[V];
         load_v<V>(f, static_cast<const W*>(a.w) + k.at, k.n);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[c][i] *= rstd * f[i];
+        for (int i = 0; i < V; ++i) v[c][i] = v[c][i] * rstd * f[i];
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[c][i] *= rstd;
@@ -158,8 +171,8 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_norm(Norm a) {
 #pragma unroll
     for (int i = 0; i < V; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[c][i]) & 0x7fffffffu);
   const float most = row_top<TPR>(top, reinterpret_cast<uint32_t*>(sh[1]));
-  // a row of zeros (or of less than the smallest normal scale holds) keeps a finite reciprocal; a NaN stays one (the comparison is false)
-  float scale = most * (1.f / 448.f);
+  // a row of zeros (or of less than the smallest normal scale holds) has something to be divided by; a NaN stays one (the comparison is false)
+  float scale = most / 448.f;
   if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;
   if (t == 0) a.scale[r] = scale;
   const float inv = 1.f / scale;
@@ -167,7 +180,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_norm(Norm a) {
 #pragma unroll
   for (int c = 0; c < NV; ++c) {
     const Chunk<V> k(t + c * TPR, a.dim);
-    if (k.used()) store_q<V>(q + k.at, v[c], inv, k.n);
+    if (k.used()) store_q<V>(q + k.at, v[c], scale, inv, k.n);
   }
 }
 

@@ -6,6 +6,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcagc_hip.so")
@@ -195,6 +196,14 @@ def rows_of(t, width):
 
 def address(t):
     return None if t is None else t.data_ptr()
+
+
+def no_tangents(name, tensors):
+    """refuses dual tensors of torch.autograd.forward_ad: a kernel's output would carry no tangent, which reads as a derivative of zero"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def launch(name, device, *args):

@@ -3,14 +3,14 @@
     out = act(scale * input @ Wg.T + bg) * (scale * input @ Wu.T + bu),   weight = [Wg; Wu] of 2n rows, act = SiLU or GELU
 
 GPU tensors -> cagc_gated_linear_* (csrc/gated.hip), one kernel for both projections, the activation and the product; fp32 / fp16 / bf16 with
-fp32 sums.  CPU tensors -> composed PyTorch.  First-order autograd (a second derivative raises)."""
+fp32 sums.  CPU tensors -> composed PyTorch.  First-order autograd (a second derivative raises, and so does forward mode on the GPU)."""
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 from torch.nn import functional as F
 
 from .. import _lib
-from .._lib import ROW_DTYPE, address, launch, rows_of
+from .._lib import ROW_DTYPE, address, launch, no_tangents, rows_of
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}      # CAGC_ACT_*
 _TYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -109,6 +109,7 @@ def gated_linear(input, weight, bias=None, activation="silu", scale=1.0):
         return _composed(z if bias is None else z + bias.to(wide), activation).to(dtype)
     if dtype not in _TYPES:
         raise RuntimeError(f"gated_linear (HIP): unsupported dtype {dtype}")
+    no_tangents("gated_linear", (input, weight, bias))
     if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GatedLinear.apply(input, weight, bias, act, float(scale), shape, n, dev)
     return _forward(input, weight, bias, act, float(scale), dtype, shape, n, dev)[0]
@@ -128,6 +129,7 @@ def gated_linear_e4m3(input, input_scale, weight, weight_scale, bias=None, activ
             raise RuntimeError(f"{name}: {what} {tuple(s.shape)} {s.dtype} on {s.device} ({tuple(want)} float32 on {input.device})")
     if torch.is_grad_enabled() and (input_scale.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad()")
+    no_tangents(name, (input, input_scale, weight, weight_scale, bias))
     if dev < 0:
         z = F.linear(input.float(), weight.float()) * input_scale[..., None] * weight_scale
         return _composed(z if bias is None else z + bias.float(), activation).to(out_dtype)

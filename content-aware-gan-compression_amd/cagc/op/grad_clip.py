@@ -39,6 +39,7 @@ def _composed_norm(tensors, code):
 
 def _launch(tensors, code, max_norm, scale, dev):
     """the norm (0-dim fp32); with `scale`, the tensors are clipped in place"""
+    _lib.no_tangents("clip_grad_norm_" if scale else "get_total_norm", tensors)
     flat, n = tensors, len(tensors)
     if not all(map(_T.is_contiguous, tensors)):
         starts = [t.data_ptr() for t in tensors if t.numel()]

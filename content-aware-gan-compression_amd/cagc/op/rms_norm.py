@@ -4,13 +4,13 @@
     h = input + residual (rounded to the type: it is returned),  out = h * (mean(h^2) + eps)^-1/2 * weight
 
 GPU tensors -> cagc_rms_norm_* (csrc/rmsnorm.hip): fp32 / fp16 / bf16, sums in fp32, weight in the input's type or fp32.  CPU tensors ->
-composed PyTorch.  First-order autograd (a second derivative raises)."""
+composed PyTorch.  First-order autograd (a second derivative raises, and so does forward mode on the GPU)."""
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .._lib import ROW_DTYPE, address, launch, rows_of
+from .._lib import ROW_DTYPE, address, launch, no_tangents, rows_of
 
 E4M3_MAX = 448.0
 _CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 3}      # the types of rows, of ROW_DTYPE
@@ -124,6 +124,7 @@ def rms_norm(input, weight=None, residual=None, eps=1e-6):
         y, h = _composed(input, weight, residual, eps)
         y = y.to(dtype)
         return y if residual is None else (y, h)
+    no_tangents("rms_norm", (input, weight, residual))
     if _needs_grad(input, weight, residual):
         return _RMSNorm.apply(input, weight, residual, eps, dev)
     out, h, _, _, _ = _forward(input, weight, residual, eps, dev, False)
@@ -143,6 +144,7 @@ def rms_norm_e4m3(input, weight=None, residual=None, eps=1e-6):
     shape, dtype, dev = _check("rms_norm_e4m3", input, weight, residual)
     if _needs_grad(input, weight, residual):
         raise RuntimeError("rms_norm_e4m3 has no backward pass: call it under torch.no_grad(), or use rms_norm")
+    no_tangents("rms_norm_e4m3", (input, weight, residual))
     if dev < 0:
         y, h = _composed(input, weight, residual, eps)
         return _quantize(y) if residual is None else (*_quantize(y), h)

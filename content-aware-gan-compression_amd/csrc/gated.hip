@@ -770,6 +770,9 @@ bool sizes_ok(int64_t rows, int64_t n, int64_t k, int dtype) {
   return rows >= 0 && n > 0 && k > 0 && rows < (1ll << 31) - 512 && n <= (1 << 26) && k * esize(dtype) <= MOST_LD;
 }
 
+// dz's rows [2n] are read along K by the tiles, so they stay within a tile's offsets too; a forward pass that saves for a backward pass is held to it as well
+bool dz_ok(int64_t n, int dtype) { return (2 * n + 16) * esize(dtype) <= MOST_LD; }
+
 // rows of a workgroup of k_dz: 8, a row a thread, while that makes few workgroups; 16 (each band writes a row of shares of db); as many more as keep the grid to 65535 of them
 int band_of(int64_t rows, int64_t n) {
   int64_t band = rows * n < (1 << 20) ? 8 : 16;
@@ -866,6 +869,7 @@ extern "C" int cagc_gated_linear_fwd(void* out, void* saved, void* ws, const voi
   CAGC_REQUIRE(act == CAGC_ACT_SILU || act == CAGC_ACT_GELU, "%s: activation %d", what, act);
   CAGC_REQUIRE(dtype == CAGC_E4M3 ? (out_dtype == CAGC_F16 || out_dtype == CAGC_BF16 || out_dtype == CAGC_F32) && !saved : out_dtype == dtype && !x_scale && !w_scale,
                "%s: output type %d for element type %d", what, out_dtype, dtype);
+  CAGC_REQUIRE(!saved || dz_ok(n, dtype), "%s: n too large for a backward pass (2n values of at most %lld bytes)", what, (long long)MOST_LD);
   if (rows == 0) return CAGC_OK;
   CAGC_REQUIRE(out && x && w, "%s: null pointer", what);
   const int64_t e = esize(dtype), kb = k * e;
@@ -913,7 +917,7 @@ extern "C" int cagc_gated_linear_bwd(void* dx, void* dw, void* db, void* ws, con
   const char* what = "cagc_gated_linear_bwd";
   CAGC_REQUIRE(dtype == CAGC_F32 || dtype == CAGC_F16 || dtype == CAGC_BF16, "%s: element type %d", what, dtype);
   CAGC_REQUIRE(sizes_ok(rows, n, k, dtype) && ldx >= k && ldw >= k && lddy >= n, "%s: bad sizes", what);
-  CAGC_REQUIRE((2 * n + 16) * esize(dtype) <= MOST_LD, "%s: n too large (2n values of at most %lld bytes)", what, (long long)MOST_LD);
+  CAGC_REQUIRE(dz_ok(n, dtype), "%s: n too large (2n values of at most %lld bytes)", what, (long long)MOST_LD);
   CAGC_REQUIRE(act == CAGC_ACT_SILU || act == CAGC_ACT_GELU, "%s: activation %d", what, act);
   CAGC_REQUIRE(rows > 0, "%s: no rows (the gradients of weight and bias are zero)", what);
   if (!dx && !dw && !db) return CAGC_OK;

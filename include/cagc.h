@@ -556,7 +556,8 @@ int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, const void* 
  * w is [2n, k]: the n gate rows, then the n up rows.  x [rows, k] and w may have rows further apart than k (ldx, ldw: elements);
  * out [rows, n] is contiguous.  dtype: CAGC_F32 / F16 / BF16, sums in fp32, one rounding to out_dtype (= dtype).
  * dtype CAGC_E4M3: x and w hold e4m3 values, x_scale [rows] and w_scale [2n] multiply their rows; out_dtype F32 / F16 / BF16, bias in
- * that type.  Any n, alignment and distance of rows; k up to 7 MiB of a row; rows 0 is a no-op.
+ * that type.  Any n, alignment and distance of rows; k up to 7 MiB of a row, n up to 2^26, with `saved` (and in the backward pass) 2n + 16 values
+ * up to 7 MiB; rows 0 is a no-op.
  * saved [nullable]: pre-activations for the backward pass: fp32 [2][rows][n]; 16-bit types: uint16 [3][rows][n] (24 bits of each).
  * ws: cagc_gated_linear_workspace bytes (0: may be null), 256-byte aligned.
  * ---------------------------------------------------------------------------------------------- */

@@ -3,7 +3,7 @@
 
 GPU tensors -> cagc_clip_grad_norm (csrc/gradnorm.hip): a launch for up to 120 tensors' norm, one that joins it, one that scales (and
 leaves at once where nothing is to be clipped); sums in 64 bits and in a fixed order; nothing waits for the host, so it can be captured.  CPU tensors ->
-composed PyTorch."""
+composed PyTorch.  On the GPU two tensors of the list must not share memory (strided views of one buffer may lie between each other)."""
 from array import array
 from operator import attrgetter
 
@@ -37,14 +37,61 @@ def _composed_norm(tensors, code):
     return s.sqrt() if code == 2 else s
 
 
+def _place(t):
+    """(first address, [(stride, count), ...] in bytes, the largest stride first, the distance of its last byte): the bytes that t's elements take"""
+    e = t.element_size()
+    dims = []
+    for s, n in [(1, e)] + sorted((s * e, n) for s, n in zip(t.stride(), t.size()) if n > 1 and s):
+        if dims and s == dims[-1][0] * dims[-1][1]:
+            dims[-1] = (dims[-1][0], dims[-1][1] * n)
+        else:
+            dims.append((s, n))
+    return t.data_ptr(), dims[::-1], _reach(dims)
+
+
+def _reach(dims):
+    return sum(s * (n - 1) for s, n in dims)
+
+
+def _meet(a, b, d, left):
+    """whether a byte of layout `a` is one of layout `b`, which begins d behind it.  The outer dimension with the larger stride goes by; of two with the same stride only the difference of their
+    indices matters, so that columns of one matrix cost the same however many rows it has.  left: steps that may be taken, then the answer is yes."""
+    if d > _reach(a) or -d > _reach(b):
+        return False
+    if not a and not b:
+        return d == 0
+    left[0] -= 1
+    if left[0] < 0:
+        return True
+    sa, sb = a[0][0] if a else 0, b[0][0] if b else 0
+    s = max(sa, sb)
+    a1, b1 = a[1:] if sa == s else a, b[1:] if sb == s else b
+    lo = -((_reach(a1) - d) // s)                # d - m s within [-reach(b1), reach(a1)]
+    hi = (d + _reach(b1)) // s
+    lo, hi = max(lo, 1 - b[0][1] if sb == s else 0), min(hi, a[0][1] - 1 if sa == s else 0)
+    return any(_meet(a1, b1, d - m * s, left) for m in range(lo, hi + 1))
+
+
+def _share_memory(tensors):
+    """whether two tensors of the list have an element's memory in common"""
+    places, open_ = sorted((_place(t) for t in tensors if t.numel()), key=lambda p: p[0]), []
+    for p in places:
+        open_ = [q for q in open_ if q[0] + q[2] >= p[0]]
+        if any(_meet(q[1], p[1], p[0] - q[0], [20000]) for q in open_):
+            return True
+        open_.append(p)
+    return False
+
+
 def _launch(tensors, code, max_norm, scale, dev):
     """the norm (0-dim fp32); with `scale`, the tensors are clipped in place"""
     _lib.no_tangents("clip_grad_norm_" if scale else "get_total_norm", tensors)
     flat, n = tensors, len(tensors)
     if not all(map(_T.is_contiguous, tensors)):
-        starts = [t.data_ptr() for t in tensors if t.numel()]
-        if len(set(starts)) < len(starts):      # (the library sees their copies)
+        if _share_memory(tensors):              # (the library sees copies)
             raise RuntimeError("cagc_clip_grad_norm: two tensors of the list share memory")
+        if scale and any(s == 0 and n > 1 for t in tensors for s, n in zip(t.stride(), t.size())):
+            raise RuntimeError("cagc_clip_grad_norm: elements of an expanded tensor share memory")
         flat = [t.contiguous() for t in tensors]
     p, sizes = array("Q", map(_T.data_ptr, flat)), array("q", map(_T.numel, flat))
     types = array("i", map(_CODES.__getitem__, map(_dtype, flat)))

@@ -359,9 +359,13 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
       if (bias) { bg = four_of(bias, n, last); bu = four_of(bias + a.np, n, last); }
 #pragma unroll
       for (int j = 0; j < K::IQ; ++j) {
-        const float q = a.sq ? a.sq[min(m0 + mw + j * 16, a.nq - 1)] : 1.f;
-        t.acc[i][j] = t.acc[i][j] * (sg * q) + bg;
-        t.acc[HI + i][j] = t.acc[HI + i][j] * (su * q) + bu;
+        if constexpr (Type<T>::size == 1) {      // one scale after the other: their product may leave fp32's range where the scaled sum does not
+          const float q = a.sq ? a.sq[min(m0 + mw + j * 16, a.nq - 1)] : 1.f;
+          t.acc[i][j] *= q;
+          t.acc[HI + i][j] *= q;
+        }
+        t.acc[i][j] = t.acc[i][j] * sg + bg;
+        t.acc[HI + i][j] = t.acc[HI + i][j] * su + bu;
       }
     }
     typedef Out<O, BQ, COLS, NT> Z;
@@ -419,10 +423,11 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
 // the gated epilogue for the (up to) four outputs [m][n .. n+3], straight to memory
 template <class O> __device__ __forceinline__ void gated_out(const Product& a, int m, int n, f32x4 g, f32x4 u) {
   const int left = a.np - n, last = a.np - 1;
-  const float q = a.alpha * (a.sq ? a.sq[m] : 1.f);
   const O* bias = static_cast<const O*>(a.bias);
-  g *= a.sp ? four_of(a.sp, n, last) * q : f32x4{q, q, q, q};
-  u *= a.sp ? four_of(a.sp + a.np, n, last) * q : f32x4{q, q, q, q};
+  if (a.sq) { g *= a.sq[m]; u *= a.sq[m]; }      // (one scale after the other, as in the tiles' epilogue)
+  g *= a.alpha;
+  u *= a.alpha;
+  if (a.sp) { g *= four_of(a.sp, n, last); u *= four_of(a.sp + a.np, n, last); }
   if (bias) { g += four_of(bias, n, last); u += four_of(bias + a.np, n, last); }
   put4(static_cast<O*>(a.out) + (int64_t)m * a.ldo + n, a.act == CAGC_ACT_SILU ? gate<CAGC_ACT_SILU>(g, u) : gate<CAGC_ACT_GELU>(g, u), left);
   if (!a.saved) return;

@@ -107,6 +107,7 @@ _PROTOS = {
     "cagc_rms_norm_bwd": [_p] * 8 + [_i64] * 5 + [_i, _i, _p],
     "cagc_gated_linear_workspace": [_p, _p] + [_i64] * 5 + [_i],
     "cagc_gated_linear_fwd": [_p] * 8 + [_i64] * 5 + [_i, _i, _i, _f, _p],
+    "cagc_gated_linear_plan": [ctypes.POINTER(ctypes.c_int)] * 3 + [_i] + [_i64] * 3 + [_i],
     "cagc_gated_linear_bwd_workspace": [_p, _p] + [_i64] * 5 + [_i] * 4,
     "cagc_gated_linear_bwd": [_p] * 8 + [_i64] * 6 + [_i, _i, _f, _p],
     "cagc_grad_norm_workspace": [_p, _i],

@@ -910,6 +910,23 @@ extern "C" int cagc_gated_linear_fwd(void* out, void* saved, void* ws, const voi
   return forward<e4m3, __bf16>(a, l, st, what);
 }
 
+extern "C" int cagc_gated_linear_plan(int* columns, int* tile_rows, int* pieces, int product, int64_t rows, int64_t n, int64_t k, int dtype) {
+  const char* what = "cagc_gated_linear_plan";
+  CAGC_REQUIRE(columns && tile_rows && pieces, "%s: null pointer", what);
+  CAGC_REQUIRE(dtype == CAGC_F32 || dtype == CAGC_F16 || dtype == CAGC_BF16 || (dtype == CAGC_E4M3 && product == 0), "%s: element type %d", what, dtype);
+  CAGC_REQUIRE(product >= 0 && product <= 2 && rows > 0 && sizes_ok(rows, n, k, dtype) && (product == 0 || dz_ok(n, dtype)), "%s: bad sizes or product", what);
+  Plan p;
+  if (product == 0) {
+    const FwdLayout l = fwd_layout(rows, n, k, true, true, dtype);
+    p = l.few ? Plan{0, 0, 1} : l.plan;
+  } else {
+    const BwdLayout l = bwd_layout(rows, n, k, true, true, dtype, product == 1, product == 2, false);
+    p = product == 1 ? l.dx : l.dw;
+  }
+  *columns = p.bp; *tile_rows = p.bq; *pieces = p.splits;
+  return CAGC_OK;
+}
+
 extern "C" int64_t cagc_gated_linear_bwd_workspace(const void* x, const void* w, int64_t rows, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int dtype, int need_dx, int need_dw,
                                                    int need_db) {
   if (!sizes_ok(rows, n, k, dtype)) return 0;

@@ -569,6 +569,9 @@ int cagc_gated_linear_fwd(void* out, void* saved /*[nullable]*/, void* ws, const
  * a fixed order: two calls give the same bits. */
 int64_t cagc_gated_linear_bwd_workspace(const void* x, const void* w, int64_t rows, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int dtype, int need_dx,
                                         int need_dw, int need_db);
+/* how a product of these sizes is cut (product 0: the forward, 1: dx, 2: dw): rows of its two operands in a tile (columns, tile_rows) and pieces of K; columns 0: the
+ * kernel for few rows.  Host arithmetic only. */
+int cagc_gated_linear_plan(int* columns, int* tile_rows, int* pieces, int product, int64_t rows, int64_t n, int64_t k, int dtype);
 int cagc_gated_linear_bwd(void* dx, void* dw, void* db, void* ws, const void* dy, const void* saved, const void* x, const void* w, int64_t rows,
                           int64_t n, int64_t k, int64_t ldx, int64_t ldw, int64_t lddy, int dtype, int act, float scale, cagc_stream_t stream);
 

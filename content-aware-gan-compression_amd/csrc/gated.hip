@@ -424,9 +424,8 @@ __global__ __launch_bounds__(WP* WQ * 64) void k_product(Product a) {
 template <class O> __device__ __forceinline__ void gated_out(const Product& a, int m, int n, f32x4 g, f32x4 u) {
   const int left = a.np - n, last = a.np - 1;
   const O* bias = static_cast<const O*>(a.bias);
-  if (a.sq) { g *= a.sq[m]; u *= a.sq[m]; }      // (one scale after the other, as in the tiles' epilogue)
-  g *= a.alpha;
-  u *= a.alpha;
+  const float q = a.alpha * (a.sq ? a.sq[m] : 1.f);
+  g *= q; u *= q;                                // (one scale after the other, as in the tiles' epilogue)
   if (a.sp) { g *= four_of(a.sp, n, last); u *= four_of(a.sp + a.np, n, last); }
   if (bias) { g += four_of(bias, n, last); u += four_of(bias + a.np, n, last); }
   put4(static_cast<O*>(a.out) + (int64_t)m * a.ldo + n, a.act == CAGC_ACT_SILU ? gate<CAGC_ACT_SILU>(g, u) : gate<CAGC_ACT_GELU>(g, u), left);

@@ -753,10 +753,17 @@ int pad_rows(const Pad* jobs, int count, hipStream_t st, const char* what) {
 
 template <class T, class O, int MQ, int C> int launch_few(Product& a, hipStream_t st, const char* what) {
   const int blocks = cdiv(a.np, C);
-  // waves that share K: more where there are few workgroups, at least 2 turns each (16 columns: 16 x 4096 -> 8192 e4m3 with 8 waves 13.9 us, with 16 15.6; 8 columns: 1 x 4096 -> 8192 bf16 26.4 and 25.6)
-  int nw = 4;
-  while (nw < 16 && blocks * nw < (C == 8 ? 8192 : 4096) && a.kbytes >= 512 * nw) nw *= 2;
-  hipLaunchKernelGGL((k_few_rows<T, O, MQ, C>), dim3(blocks), dim3(nw * 64), (size_t)nw / 2 * MQ * (C / 8) * 64 * sizeof(f32x4), st, a);      // (at most 64 KB)
+  // Waves that share K, at least two turns each: mostly eight.  16 columns: four where a CU has more than one workgroup, rows are up to 8 KB and not both short and of a single product.  8 columns: sixteen
+  // where rows are 8 KB and more and a CU has at most three workgroups, four where it has eight and rows are up to 8 KB.  With 4 / 8 / 16 waves, us (weights from HBM): 16 columns, 16 x 8192 -> 4096 bf16
+  // 43.4 / 33.2 / 33.7, 16 x 1024 -> 8192 bf16 11.3 / 9.9 / 12.1, 32 x 4096 -> 5120 bf16 35.6 / 38.9 / 40.3, 16 x 8192 -> 8192 e4m3 26.5 / 28.6 / 30.9; 8 columns, 1 x 2048 -> 2048 bf16 7.5 / 5.9 / 6.1,
+  // 1 x 4096 -> 4096 bf16 14.7 / 14.0 / 13.6, 1 x 4096 -> 8192 fp32 64.5 / 46.3 / 49.1, 1 x 4096 -> 16384 bf16 46.8 / 50.0 / 49.2.  Over 378 sizes (1 to 32 rows, n 512 to 24576, rows of 1 to 16 KB,
+  // three types) the rule's choice takes 0.7 % (8 columns 1.5 %) longer than the best of the three in the mean, 7 (15) % at worst; eight everywhere would take 2.4 (2.2) % longer.
+  int nw = 8;
+  if (C == 16 && blocks > 256 && a.kbytes <= 8192 && (MQ > 1 || a.kbytes > 4096)) nw = 4;
+  if (C == 8 && blocks <= 768 && a.kbytes >= 8192) nw = 16;
+  if (C == 8 && blocks >= 2048 && a.kbytes <= 8192) nw = 4;
+  if (a.kbytes < 256 * nw) nw = 4;
+  hipLaunchKernelGGL((k_few_rows<T, O, MQ, C>), dim3(blocks), dim3(nw * 64), (size_t)nw / 2 * MQ * (C / 8) * 64 * sizeof(f32x4), st, a);      // (at most 32 KB)
   return check_launch(what);
 }
 template <class T, class O> int few_rows(Product& a, hipStream_t st, const char* what) {

@@ -197,15 +197,15 @@ struct NormBwd {
   int dim;
 };
 
-// A workgroup takes rows blockIdx.x * RPB, + gridDim.x * RPB, ...: a thread keeps its columns of w and of dw in registers throughout.
+// A workgroup takes rows blockIdx.x * RPB, + gridDim.x * RPB, ...: a thread keeps its columns of w and of dw in registers throughout.  16-bit rows of more than 16384 elements, four chunks of 1024 threads,
+// want more than the 128 registers of a lane there: some 95 of them spill.  Reading w anew for each row (it stays in L2) still spills 75 and is slower: 2048 x 32768 bf16 467 us, so 423.
 template <class T, class W, int TPR, int NV>
 __global__ __launch_bounds__(threads_of(TPR)) void k_rms_norm_bwd(NormBwd a) {
   constexpr int V = Row<T>::V, RPB = threads_of(TPR) / TPR;
   __shared__ float sh[2][TPR / 64];
   __shared__ float join[RPB > 1 ? NV * V * TPR : 1];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-  constexpr bool KEEP = NV * V * TPR <= 16384;      // wider rows read w again for each row (it stays in L2) rather than spill
-  float w[KEEP ? NV : 1][V], dw[NV][V];
+  float w[NV][V], dw[NV][V];
   auto weight = [&](int c, float (&f)[V]) {
     const Chunk<V> k(t + c * TPR, a.dim);
     if (a.w) { load_v<V>(f, static_cast<const W*>(a.w) + k.at, k.n); return; }
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_norm_bwd(NormBwd a) {
   };
 #pragma unroll
   for (int c = 0; c < NV; ++c) {
-    if (KEEP) weight(c, w[KEEP ? c : 0]);
+    weight(c, w[c]);
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[c][i] = 0.f;
   }
@@ -233,12 +233,11 @@ __global__ __launch_bounds__(threads_of(TPR)) void k_rms_norm_bwd(NormBwd a) {
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const Chunk<V> k(t + c * TPR, a.dim);
-      if (!KEEP) weight(c, w[0]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         n[c][i] *= rstd;
         dw[c][i] += d[c][i] * n[c][i];
-        d[c][i] *= w[KEEP ? c : 0][i];
+        d[c][i] *= w[c][i];
         s += i >= k.skip ? d[c][i] * n[c][i] : 0.f;
       }
     }

@@ -601,7 +601,9 @@ __global__ __launch_bounds__(256) void k_pad_rows(Pad a, Pad b) {
 }
 
 // dz [rows, ldz] from the saved pre-activations and dy (zeros behind 2n), 8 or 4 columns a thread (16 bytes of dz), and the column sums of a band of rows
-// for db.  Bound by its bytes: dy, 3 planes of 16 bits (2 of fp32) and dz's two halves.
+// for db (in fp32, before dz is rounded).  dz is rounded to the type, because the matrix cores multiply 16-bit operands; with the 24 bits of the pre-activations the gradients' error in bf16 is 1.4 times that
+// of one final rounding (dz as a sum of two values of the type would take twice the products).  In fp16 a |dz| above 65504 is infinite and one below 2^-14 loses bits, as the gradient of a
+// pre-activation in fp16 does: loss scaling has to keep it in range.  Bound by its bytes: dy, 3 planes of 16 bits (2 of fp32) and dz's two halves.
 template <class T> __global__ __launch_bounds__(256) void k_dz(T* __restrict__ z, float* __restrict__ dbpart, const T* __restrict__ dy, int64_t lddy, const void* __restrict__ saved,
                                                               int rows, int n, int64_t ldz, int act, int band) {
   constexpr int V = 16 / (int)sizeof(T), GROUPS = 32;      // 32 threads side by side, 8 rows at a time

@@ -556,7 +556,8 @@ int cagc_rms_norm_bwd(void* dx, void* dw, void* ws, const void* dy, const void* 
  * w is [2n, k]: the n gate rows, then the n up rows.  x [rows, k] and w may have rows further apart than k (ldx, ldw: elements);
  * out [rows, n] is contiguous.  dtype: CAGC_F32 / F16 / BF16, sums in fp32, one rounding to out_dtype (= dtype).
  * dtype CAGC_E4M3: x and w hold e4m3 values, x_scale [rows] and w_scale [2n] multiply their rows; out_dtype F32 / F16 / BF16, bias in
- * that type.  Any n, alignment and distance of rows; k up to 7 MiB of a row, n up to 2^26, with `saved` (and in the backward pass) 2n + 16 values
+ * that type; the matrix cores keep 14 bits below the largest of 8 neighbouring products (sums of normal values to 1.5e-5 of their size).
+ * Any n, alignment and distance of rows; k up to 7 MiB of a row, n up to 2^26, with `saved` (and in the backward pass) 2n + 16 values
  * up to 7 MiB; rows 0 is a no-op.
  * saved [nullable]: pre-activations for the backward pass: fp32 [2][rows][n]; 16-bit types: uint16 [3][rows][n] (24 bits of each).
  * ws: cagc_gated_linear_workspace bytes (0: may be null), 256-byte aligned.
@@ -565,7 +566,8 @@ int64_t cagc_gated_linear_workspace(const void* x, const void* w, int64_t rows, 
 int cagc_gated_linear_fwd(void* out, void* saved /*[nullable]*/, void* ws, const void* x, const void* w, const void* bias /*[nullable]*/,
                           const float* x_scale /*[nullable]*/, const float* w_scale /*[nullable]*/, int64_t rows, int64_t n, int64_t k,
                           int64_t ldx, int64_t ldw, int dtype, int out_dtype, int act, float scale, cagc_stream_t stream);
-/* dx [rows, k], dw [2n, k], db [2n] (each nullable: not wanted), contiguous, in dtype; dy [rows, n] with rows lddy apart.  rows > 0.  Every sum runs in
+/* dx [rows, k], dw [2n, k], db [2n] (each nullable: not wanted), contiguous, in dtype; dy [rows, n] with rows lddy apart.  rows > 0.  The pre-activations'
+ * gradients are rounded to dtype before both products (fp16: magnitudes above 65504 become infinite).  Every sum runs in
  * a fixed order: two calls give the same bits. */
 int64_t cagc_gated_linear_bwd_workspace(const void* x, const void* w, int64_t rows, int64_t n, int64_t k, int64_t ldx, int64_t ldw, int dtype, int need_dx,
                                         int need_dw, int need_db);

@@ -37,8 +37,16 @@ def _composed_norm(tensors, code):
     return s.sqrt() if code == 2 else s
 
 
-def _place(t):
-    """(first address, [(stride, count), ...] in bytes, the largest stride first, the distance of its last byte): the bytes that t's elements take"""
+def _span(t):
+    """(first address, distance of the last byte, t)"""
+    e = t.element_size()
+    if t.is_contiguous():
+        return t.data_ptr(), t.numel() * e - 1, t
+    return t.data_ptr(), sum(s * (n - 1) for s, n in zip(t.stride(), t.size())) * e + e - 1, t
+
+
+def _layout_of(t):
+    """[(stride, count), ...] in bytes, the largest stride first: the bytes that t's elements take, from its first address on"""
     e = t.element_size()
     dims = []
     for s, n in [(1, e)] + sorted((s * e, n) for s, n in zip(t.stride(), t.size()) if n > 1 and s):
@@ -46,7 +54,7 @@ def _place(t):
             dims[-1] = (dims[-1][0], dims[-1][1] * n)
         else:
             dims.append((s, n))
-    return t.data_ptr(), dims[::-1], _reach(dims)
+    return dims[::-1]
 
 
 def _reach(dims):
@@ -74,10 +82,10 @@ def _meet(a, b, d, left):
 
 def _share_memory(tensors):
     """whether two tensors of the list have an element's memory in common"""
-    places, open_ = sorted((_place(t) for t in tensors if t.numel()), key=lambda p: p[0]), []
-    for p in places:
-        open_ = [q for q in open_ if q[0] + q[2] >= p[0]]
-        if any(_meet(q[1], p[1], p[0] - q[0], [20000]) for q in open_):
+    open_ = []                  # those that reach beyond where the next one begins
+    for p in sorted((_span(t) for t in tensors if t.numel()), key=lambda p: p[0]):
+        open_ = [q for q in open_ if q[0] + q[1] >= p[0]]
+        if open_ and any(_meet(_layout_of(q[2]), _layout_of(p[2]), p[0] - q[0], [20000]) for q in open_):
             return True
         open_.append(p)
     return False
